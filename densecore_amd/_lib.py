@@ -1,4 +1,5 @@
-"""ctypes binding of ``libdcattn.so`` (the C ABI in ``include/dc_attn.h`` and ``include/dc_math.h``).
+"""ctypes binding of ``libdcattn.so`` (the C ABI in ``include/dc_attn.h``, ``dc_math.h`` and
+``dc_rotary.h``).
 
 The library is built in-tree (``densecore_amd/libdcattn.so``) by ``densecore_amd.build``.
 If it is missing, every entry point raises: there is no CPU fallback on this path.
@@ -13,7 +14,7 @@ DC_OK, DC_INVALID_ARGUMENT, DC_UNSUPPORTED, DC_EXECUTION_FAILED = 0, 1, 2, 3
 DC_F32, DC_BF16 = 0, 1
 DC_FLAG_CONSISTENT_SCORES = 1
 
-# Every symbol include/dc_attn.h and include/dc_math.h declare.
+# Every symbol the headers under include/ declare.
 EXPORTS = ("dc_abi_version", "dc_last_error",
            "dc_sdpa_fwd_workspace_size", "dc_sdpa_fwd",
            "dc_sdpa_bwd_workspace_size", "dc_sdpa_bwd",
@@ -22,7 +23,8 @@ EXPORTS = ("dc_abi_version", "dc_last_error",
            "dc_bmm", "dc_softmax_fwd", "dc_softmax_bwd",
            "dc_mt19937_seed", "dc_mt19937_advance", "dc_mt19937_table_bytes",
            "dc_mt19937_table_init", "dc_bernoulli_max_draws", "dc_bernoulli_workspace_size",
-           "dc_bernoulli", "dc_dropout_apply")
+           "dc_bernoulli", "dc_dropout_apply",
+           "dc_rotary_fwd", "dc_rotary_bwd_workspace_size", "dc_rotary_bwd")
 
 
 class Desc(ctypes.Structure):
@@ -61,6 +63,16 @@ class SoftmaxDesc(ctypes.Structure):
                 ("q_len", ctypes.c_int64), ("mask_stride_b", ctypes.c_int64),
                 ("mask_stride_h", ctypes.c_int64), ("mask_stride_l", ctypes.c_int64),
                 ("safe", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class RotaryDesc(ctypes.Structure):
+    """``dc_rotary_desc``."""
+    _fields_ = ([(n, ctypes.c_int64) for n in ("batch", "heads", "kv_heads", "q_len", "head_dim", "rotary_dim")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "weight_dtype", "interleaved", "norm", "pos_bytes",
+                                                 "reserved")]
+                + [(n, ctypes.c_int64) for n in ("offset", "pos_stride_b", "pos_stride_l")]
+                + [("magnitude", ctypes.c_double), ("eps", ctypes.c_double)]
+                + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "grad_q_stride", "grad_k_stride")])
 
 
 _lib = None
@@ -107,9 +119,16 @@ def lib():
         L.dc_bernoulli_workspace_size.restype = SZ
         L.dc_bernoulli.argtypes = [P, P, I64P, I64P, ctypes.c_int64, ctypes.c_double, P, P, SZ, P]
         L.dc_dropout_apply.argtypes = [P, ctypes.c_int64, ctypes.c_float, P, P, P]
-        for name in ("dc_sdpa_fwd", "dc_sdpa_bwd", "dc_sdpa_decode", "dc_softmax_fwd",
+        RD = ctypes.POINTER(RotaryDesc)
+        L.dc_rotary_fwd.argtypes = [RD, P, P, P, P, P, P, P, P, P]
+        L.dc_rotary_bwd_workspace_size.argtypes = [RD]
+        L.dc_rotary_bwd_workspace_size.restype = SZ
+        L.dc_rotary_bwd.argtypes = [RD] + [P] * 13 + [SZ, P]
+        for name in ("dc_rotary_fwd", "dc_rotary_bwd",
+                     "dc_sdpa_fwd", "dc_sdpa_bwd", "dc_sdpa_decode", "dc_softmax_fwd",
                      "dc_softmax_bwd", "dc_mt19937_advance", "dc_mt19937_table_init",
-                     "dc_bernoulli", "dc_dropout_apply"):
+                     "dc_bernoulli", "dc_dropout_apply",
+           "dc_rotary_fwd", "dc_rotary_bwd_workspace_size", "dc_rotary_bwd"):
             getattr(L, name).restype = ctypes.c_int
         _lib = L
     return _lib

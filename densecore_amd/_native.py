@@ -12,6 +12,7 @@ ordered on torch's current stream of the tensors' device.
 ``_flash_attention`` at L = 1 without causal masking.
 """
 import collections
+import contextlib
 import math
 
 import torch
@@ -309,6 +310,109 @@ def _dropout_apply(bits, x, scale):
     _lib.check(_lib.lib().dc_dropout_apply(_ptr(bits), x.numel(), float(scale), _ptr(x), _ptr(y),
                                            _stream(x.device)))
     return y
+
+
+def _on(dev):
+    """The launches of a call go to its tensors' device, whichever is current."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _unit_rows(t):
+    """``t`` with unit stride along its last dim (a copy only where it has none)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _rotary_desc(q, k, inv_freq, positions, offset, interleaved, magnitude, eps, weights, grads=(None, None)):
+    """Checks the arguments of the rotation; returns its descriptor (``dc_rotary_desc``)."""
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("rotary takes (B, H, L, E) tensors")
+    B, H, L, E = q.shape
+    if k is not None and (k.shape[0], k.shape[2], k.shape[3]) != (B, L, E):
+        raise ValueError("rotary query and key shapes do not match")
+    dev = q.device
+    if dev.type != "cuda":
+        raise ValueError("rotary tensors must be on the GPU")
+    if q.dtype not in _DTYPES:
+        raise ValueError("rotary takes float32 or bfloat16 tensors")
+    for t in (k, *grads):
+        if t is not None and (t.device != dev or t.dtype != q.dtype):
+            raise ValueError("rotary query and key must share one device and dtype")
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or inv_freq.device != dev:
+        raise ValueError("rotary inv_freq must be a float64 vector on the tensors' device")
+    if 2 * inv_freq.shape[0] > E:
+        raise ValueError("rotary inv_freq turns more dims than the head has")
+    wtype = _DTYPES[q.dtype]
+    for w in weights or ():
+        if w is None:
+            continue
+        if tuple(w.shape) != (E,) or w.dtype not in _DTYPES or w.device != dev:
+            raise ValueError("norm weights must be float32 or bfloat16 vectors of head_dim values on the "
+                             "tensors' device")
+    given = {w.dtype for w in weights or () if w is not None}
+    if len(given) > 1:
+        raise ValueError("norm weights must share one dtype")
+    for dtype in given:
+        wtype = _DTYPES[dtype]
+    pos_bytes, ps = 0, (0, 0)
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != dev:
+            raise ValueError("rotary positions must be int32 or int64 on the tensors' device")
+        if tuple(positions.shape) not in ((L,), (B, L), (1, L)):
+            raise ValueError("rotary positions must be (L,) or (B, L)")
+        if offset:
+            raise ValueError("rotary takes positions or an offset, not both")
+        pos_bytes = positions.element_size()
+        ps = (positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0, positions.stride(-1))
+    S3 = _lib.ctypes.c_int64 * 3
+
+    def strides(t):
+        return S3(*t.stride()[:3]) if t is not None else S3()
+    return _lib.RotaryDesc(B, H, 0 if k is None else k.shape[1], L, E, 2 * inv_freq.shape[0], _DTYPES[q.dtype],
+                           wtype, int(bool(interleaved)), int(weights is not None), pos_bytes, 0, int(offset), *ps,
+                           float(magnitude), float(eps), strides(q), strides(k), strides(grads[0]), strides(grads[1]))
+
+
+def _rotary(q, k, inv_freq, positions=None, offset=0, interleaved=False, magnitude=1.0, weights=None, eps=0.0):
+    """``dc_rotary_fwd``: (q, k) turned by their positions, contiguous; ``weights`` (a pair, either
+    None) asks for the norm of each head first.  ``k`` may be None."""
+    q, k = _unit_rows(q), None if k is None else _unit_rows(k)
+    if weights is not None:
+        weights = tuple(None if w is None else w.contiguous() for w in weights)
+    d = _rotary_desc(q, k, inv_freq, positions, offset, interleaved, magnitude, eps, weights)
+    inv_freq, dev = inv_freq.contiguous(), q.device
+    qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    ko = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+    wq, wk = weights or (None, None)
+    with _on(dev):
+        _lib.check(_lib.lib().dc_rotary_fwd(d, _ptr(q), _ptr(k), _ptr(wq), _ptr(wk), _ptr(inv_freq),
+                                            _ptr(positions), _ptr(qo), _ptr(ko), _stream(dev)))
+    return qo, ko
+
+
+def _rotary_backward(grad_q, grad_k, q, k, inv_freq, positions=None, offset=0, interleaved=False, magnitude=1.0,
+                     weights=None, eps=0.0, weight_grads=(False, False)):
+    """``dc_rotary_bwd``: (dq, dk, dq_weight, dk_weight), None for what there is none of.  Without
+    ``weights`` q and k only give the shapes."""
+    grad_q, grad_k = _unit_rows(grad_q), None if grad_k is None else _unit_rows(grad_k)
+    if weights is not None:
+        q, k = _unit_rows(q), None if k is None else _unit_rows(k)
+        weights = tuple(None if w is None else w.contiguous() for w in weights)
+    d = _rotary_desc(q, k, inv_freq, positions, offset, interleaved, magnitude, eps, weights, (grad_q, grad_k))
+    if grad_q.shape != q.shape or (k is not None and (grad_k is None or grad_k.shape != k.shape)):
+        raise ValueError("rotary backward shapes do not match")
+    inv_freq, dev = inv_freq.contiguous(), q.device
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    dk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+    wq, wk = weights or (None, None)
+    dwq, dwk = (torch.empty_like(w) if want and w is not None else None for w, want in zip((wq, wk), weight_grads))
+    x = (q, k) if weights is not None else (None, None)
+    L_ = _lib.lib()
+    with _on(dev):
+        ws = _workspace(L_.dc_rotary_bwd_workspace_size(d), dev) if dwq is not None or dwk is not None else None
+        _lib.check(L_.dc_rotary_bwd(d, _ptr(grad_q), _ptr(grad_k), _ptr(x[0]), _ptr(x[1]), _ptr(wq), _ptr(wk),
+                                    _ptr(inv_freq), _ptr(positions), _ptr(dq), _ptr(dk), _ptr(dwq), _ptr(dwk),
+                                    _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev)))
+    return dq, dk, dwq, dwk
 
 
 def default_scale(head_dim):

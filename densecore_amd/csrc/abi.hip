@@ -1,4 +1,4 @@
-// The C ABI declared in include/dc_attn.h and include/dc_math.h: argument checks with the reference's messages,
+// The C ABI declared in include/dc_attn.h, include/dc_math.h and include/dc_rotary.h: argument checks with the reference's messages,
 // scale computation, workspace carving, and dispatch to the kernel launchers.
 //
 // Checks follow the reference boundary (src/lib.rs:555-580 attention_dims, :594-607
@@ -17,7 +17,9 @@
 #include "common.hpp"
 #include "dc_attn.h"
 #include "dc_math.h"
+#include "dc_rotary.h"
 #include "params.hpp"
+#include "rotary.hpp"
 
 namespace dc {
 namespace {
@@ -774,6 +776,111 @@ dc_status dc_dropout_apply(const uint32_t *keep_bits, int64_t n, float scale, co
         return fail(DC_INVALID_ARGUMENT, "dropout got a null pointer");
     if (n > (int64_t)256 * INT32_MAX) return fail(DC_UNSUPPORTED, "dropout count exceeds 2^39");
     return launched(dc::mt::launch_dropout_apply(keep_bits, n, scale, x, y, static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"
+
+namespace {
+
+dc_status check_rotary(const dc_rotary_desc *d, const double *inv_freq, const void *positions, dc::RotArgs *a) {
+    if (d == nullptr) return fail(DC_INVALID_ARGUMENT, "rotary descriptor is null");
+    const int64_t dims[5] = {d->batch, d->heads, d->kv_heads, d->q_len, d->head_dim};
+    for (int64_t x : dims)
+        if (x < 0) return fail(DC_INVALID_ARGUMENT, "rotary takes (B, H, L, E) tensors");
+    for (int64_t x : dims)
+        if (x > INT32_MAX / 2) return fail(DC_UNSUPPORTED, "rotary dimension exceeds 2^30");
+    if (d->head_dim > DC_ROTARY_MAX_HEAD_DIM) return fail(DC_UNSUPPORTED, "rotary takes head_dim up to 512");
+    if (d->rotary_dim < 0 || d->rotary_dim % 2 != 0 || d->rotary_dim > d->head_dim)
+        return fail(DC_INVALID_ARGUMENT, "rotary_dim must be even and at most head_dim");
+    if ((d->dtype != DC_F32 && d->dtype != DC_BF16) || (d->weight_dtype != DC_F32 && d->weight_dtype != DC_BF16))
+        return fail(DC_INVALID_ARGUMENT, "rotary dtype must be float32 or bfloat16");
+    if (d->pos_bytes != 0 && d->pos_bytes != 4 && d->pos_bytes != 8)
+        return fail(DC_INVALID_ARGUMENT, "rotary positions must be int32 or int64");
+    if (d->reserved != 0) return fail(DC_INVALID_ARGUMENT, "rotary descriptor's reserved field must be 0");
+    for (int i = 0; i < 3; ++i)
+        if (d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->grad_q_stride[i] < 0 || d->grad_k_stride[i] < 0)
+            return fail(DC_INVALID_ARGUMENT, "rotary strides must be non-negative");
+    const int64_t tokens = d->batch * d->q_len;
+    if (tokens > 0 && ((d->rotary_dim > 0 && inv_freq == nullptr) || (d->pos_bytes != 0 && positions == nullptr)))
+        return fail(DC_INVALID_ARGUMENT, "rotary got a null pointer");
+    *a = dc::RotArgs{};
+    a->freq = inv_freq;
+    a->pos = positions;
+    a->pos_bytes = d->pos_bytes;
+    a->offset = d->offset, a->pos_sb = d->pos_stride_b, a->pos_sl = d->pos_stride_l;
+    a->tokens = tokens;
+    a->L = (int)d->q_len, a->E = (int)d->head_dim, a->R = (int)d->rotary_dim;
+    a->magnitude = (float)d->magnitude, a->eps = (float)d->eps;
+    a->interleaved = d->interleaved != 0, a->norm = d->norm != 0;
+    a->w_bf16 = d->weight_dtype == DC_BF16;
+    a->t[0].heads = (int)d->heads, a->t[1].heads = (int)d->kv_heads;
+    for (int i = 0; i < 3; ++i) {
+        a->t[0].xs[i] = d->q_stride[i], a->t[1].xs[i] = d->k_stride[i];
+        a->t[0].gs[i] = d->grad_q_stride[i], a->t[1].gs[i] = d->grad_k_stride[i];
+    }
+    return ok();
+}
+
+size_t rotary_part(const dc_rotary_desc *d) { return round_up((size_t)dc::kRotMaxBlocks * d->head_dim * sizeof(float)); }
+
+}  // namespace
+
+extern "C" {
+
+dc_status dc_rotary_fwd(const dc_rotary_desc *d, const void *q, const void *k, const void *q_weight,
+                        const void *k_weight, const double *inv_freq, const void *positions, void *q_out,
+                        void *k_out, void *stream) {
+    dc::RotArgs a;
+    dc_status st = check_rotary(d, inv_freq, positions, &a);
+    if (st != DC_OK) return st;
+    if (!a.norm && (q_weight || k_weight)) return fail(DC_INVALID_ARGUMENT, "rotary takes weights with norm only");
+    const int64_t n = a.tokens * a.E;
+    if (!present(q, n * a.t[0].heads) || !present(q_out, n * a.t[0].heads) || !present(k, n * a.t[1].heads) ||
+        !present(k_out, n * a.t[1].heads))
+        return fail(DC_INVALID_ARGUMENT, "rotary got a null pointer");
+    if (n == 0 || a.t[0].heads + a.t[1].heads == 0) return ok();
+    a.t[0].x = q, a.t[0].w = q_weight, a.t[0].out = q_out;
+    a.t[1].x = k, a.t[1].w = k_weight, a.t[1].out = k_out;
+    return launched(dc::launch_rotary(a, d->dtype == DC_BF16, false, static_cast<hipStream_t>(stream)));
+}
+
+size_t dc_rotary_bwd_workspace_size(const dc_rotary_desc *d) {
+    dc::RotArgs a;
+    if (d == nullptr || !d->norm) return 0;
+    if (check_rotary(d, reinterpret_cast<const double *>(d), d, &a) != DC_OK) return 0;
+    return 2 * rotary_part(d);
+}
+
+dc_status dc_rotary_bwd(const dc_rotary_desc *d, const void *grad_q, const void *grad_k, const void *q,
+                        const void *k, const void *q_weight, const void *k_weight, const double *inv_freq,
+                        const void *positions, void *dq, void *dk, void *dq_weight, void *dk_weight,
+                        void *workspace, size_t workspace_bytes, void *stream) {
+    dc::RotArgs a;
+    dc_status st = check_rotary(d, inv_freq, positions, &a);
+    if (st != DC_OK) return st;
+    if (!a.norm && (q_weight || k_weight || dq_weight || dk_weight))
+        return fail(DC_INVALID_ARGUMENT, "rotary takes weights with norm only");
+    const int64_t nq = a.tokens * a.E * a.t[0].heads, nk = a.tokens * a.E * a.t[1].heads;
+    if (!present(grad_q, nq) || !present(dq, nq) || !present(grad_k, nk) || !present(dk, nk) ||
+        (a.norm && (!present(q, nq) || !present(k, nk))))
+        return fail(DC_INVALID_ARGUMENT, "rotary got a null pointer");
+    a.t[0].g = grad_q, a.t[0].out = dq, a.t[1].g = grad_k, a.t[1].out = dk;
+    hipStream_t strm = static_cast<hipStream_t>(stream);
+    if (!a.norm) {
+        if (nq + nk == 0) return ok();
+        return launched(dc::launch_rotary(a, d->dtype == DC_BF16, true, strm));
+    }
+    a.t[0].x = q, a.t[0].w = q_weight, a.t[1].x = k, a.t[1].w = k_weight;
+    a.dw[0] = dq_weight, a.dw[1] = dk_weight;
+    if (dq_weight || dk_weight) {
+        if (workspace == nullptr || workspace_bytes < 2 * rotary_part(d))
+            return fail(DC_INVALID_ARGUMENT, "rotary backward workspace is too small");
+        float *w = static_cast<float *>(workspace);
+        if (dq_weight) a.part[0] = w;
+        if (dk_weight) a.part[1] = w + rotary_part(d) / sizeof(float);
+    }
+    if (a.E == 0) return ok();
+    return launched(dc::launch_rotary_norm_bwd(a, d->dtype == DC_BF16, strm));
 }
 
 }  // extern "C"

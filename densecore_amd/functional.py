@@ -289,6 +289,128 @@ def flash_decode(query, key, value, scale=None):
     return _native._flash_decode(query, key, value, None if scale is None else float(scale))[0]
 
 
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, original_length=None, beta_fast=32.0,
+                       beta_slow=1.0, device=None):
+    """``(inv_freq, magnitude)`` for ``rotary_embedding`` and ``qk_norm_rotary``: the angle per position
+    of each of ``rotary_dim / 2`` pairs (float64) and the factor on the turned values.
+
+    Plain: ``base ** (-2 i / rotary_dim)``.  For contexts ``factor`` times as long as the trained one,
+    ``scaling`` is ``"linear"`` (positions divided by the factor), ``"ntk"`` (the base times ``factor **
+    (R / (R - 2))``, so that the slowest pair is divided by the factor and the fastest kept) or ``"yarn"``
+    (Peng et al., "YaRN", 2023): pairs that turn more than ``beta_fast`` times over ``original_length``
+    positions are kept, those that turn less than ``beta_slow`` times divided by the factor, in between a
+    ramp, and the magnitude is ``0.1 ln(factor) + 1``."""
+    if isinstance(rotary_dim, bool) or not isinstance(rotary_dim, numbers.Integral) or rotary_dim < 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be an even number")
+    if not base > 1.0 or not factor >= 1.0:
+        raise ValueError("rotary base must be above 1 and factor at least 1")
+    R = int(rotary_dim)
+    i = torch.arange(R // 2, dtype=torch.float64)
+    magnitude = 1.0
+    if scaling == "ntk" and R > 2:
+        base = base * factor ** (R / (R - 2))
+    freq = torch.tensor(float(base), dtype=torch.float64) ** (-2.0 * i / max(R, 1))
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        if original_length is None or original_length <= 0:
+            raise ValueError("yarn scaling takes the trained length as original_length")
+        if not beta_fast > beta_slow > 0:
+            raise ValueError("yarn scaling takes beta_fast above beta_slow above 0")
+
+        def pair(turns):
+            return R * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), R - 1)
+        ramp = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
+        freq = freq / factor * ramp + freq * (1 - ramp)
+        magnitude = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError("rotary scaling must be None, 'linear', 'ntk' or 'yarn'")
+    return freq.to(device), magnitude
+
+
+class _Rotary(torch.autograd.Function):
+    """The rotation, with or without the norm (``weights`` None: without); its gradient takes nothing
+    but the positions without the norm, and the inputs again with it."""
+
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, norm, inv_freq, positions, args, eps):
+        weights = (wq, wk) if norm else None
+        ctx.save_for_backward(*(q, k, wq, wk) if norm else (None,) * 4, inv_freq, positions)
+        ctx.norm, ctx.args, ctx.eps, ctx.has_k = norm, args, eps, k is not None
+        ctx.like = [None if t is None else (t.shape, t.dtype, t.device) for t in (q, k)]
+        return _native._rotary(q, k, inv_freq, positions, *args, weights, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, wq, wk, inv_freq, positions = ctx.saved_tensors
+        if not ctx.norm:
+            q, k = gq, gk if ctx.has_k else None
+        need = ctx.needs_input_grad
+        dq, dk, dwq, dwk = _native._rotary_backward(
+            gq, gk if ctx.has_k else None, q, k, inv_freq, positions, *ctx.args, (wq, wk) if ctx.norm else None,
+            ctx.eps, (need[2], need[3]))
+        return dq, dk, dwq, dwk, None, None, None, None, None
+
+
+def _turn_args(offset, interleaved, magnitude):
+    if isinstance(offset, bool) or not isinstance(offset, numbers.Integral):
+        raise TypeError("rotary offset must be an int")
+    if type(interleaved) is not bool:
+        raise TypeError("interleaved must be a bool")
+    if isinstance(magnitude, bool) or not isinstance(magnitude, numbers.Real):
+        raise TypeError("rotary magnitude must be real")
+    return int(offset), interleaved, float(magnitude)
+
+
+def _check_tensors(what, **tensors):
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what} {name} must be a Tensor")
+
+
+def rotary_embedding(query, key, inv_freq, positions=None, offset=0, interleaved=False, magnitude=1.0):
+    """Queries (B, H, L, E) and keys (B, Hkv, L, E) turned by their positions: ``(query, key)``, contiguous.
+
+    Token (b, l) stands at ``positions[b, l]`` (int32 or int64, (L,) or (B, L)), or at ``offset + l``.
+    Pair i of a head's first ``2 len(inv_freq)`` dims is turned by the angle position x ``inv_freq[i]``
+    (float64, ``rotary_frequencies``) and multiplied by ``magnitude``; pairs are (i, i + len(inv_freq)), or
+    (2i, 2i + 1) when ``interleaved``; the dims behind them are passed on.  Float32 or bf16 in any strides
+    (a projection's (B, L, H, E) is transposed on the way); angles are formed in float64.  ``key`` may be
+    None: then the turned query alone is returned.  No counterpart in the reference."""
+    _check_tensors("rotary", query=query, inv_freq=inv_freq, **({} if key is None else {"key": key}),
+                   **({} if positions is None else {"positions": positions}))
+    args = _turn_args(offset, interleaved, magnitude)
+    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
+        q, k = _Rotary.apply(query, key, None, None, False, inv_freq, positions, args, 0.0)
+    else:
+        q, k = _native._rotary(query, key, inv_freq, positions, *args)
+    return q if key is None else (q, k)
+
+
+def qk_norm_rotary(query, key, query_weight, key_weight, inv_freq, positions=None, offset=0, interleaved=False,
+                   magnitude=1.0, eps=1e-6):
+    """``rotary_embedding`` of each head's queries and keys divided by their root mean square:
+    ``x / sqrt(mean(x^2) + eps) * weight`` over the head's E dims, then turned, in one pass.
+
+    The weights are (E,) vectors, float32 or bf16, shared by the heads (None: no weight); with an empty
+    ``inv_freq`` there is the norm alone.  Gradients: queries, keys and weights, the weights' summed in a
+    fixed order.  No counterpart in the reference."""
+    _check_tensors("rotary", query=query, key=key, inv_freq=inv_freq,
+                   **({} if positions is None else {"positions": positions}),
+                   **{n: w for n, w in (("query_weight", query_weight), ("key_weight", key_weight)) if w is not None})
+    args = _turn_args(offset, interleaved, magnitude)
+    if isinstance(eps, bool) or not isinstance(eps, numbers.Real):
+        raise TypeError("norm eps must be real")
+    if not eps >= 0:
+        raise ValueError("norm eps must not be negative")
+    leaves = (query, key, query_weight, key_weight)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
+        return _Rotary.apply(*leaves, True, inv_freq, positions, args, float(eps))
+    return _native._rotary(query, key, inv_freq, positions, *args, (query_weight, key_weight), float(eps))
+
+
 def _float_mask(mask):
     """MHA masks (``functional.py:391-397``): a bool mask is True where attention is NOT
     allowed (-inf); a float mask is added."""
