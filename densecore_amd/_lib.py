@@ -1,5 +1,5 @@
-"""ctypes binding of ``libdcattn.so`` (the C ABI in ``include/dc_attn.h``, ``dc_math.h`` and
-``dc_rotary.h``).
+"""ctypes binding of ``libdcattn.so`` (the C ABI in ``include/dc_attn.h``, ``dc_math.h``,
+``dc_rotary.h`` and ``dc_window.h``).
 
 The library is built in-tree (``densecore_amd/libdcattn.so``) by ``densecore_amd.build``.
 If it is missing, every entry point raises: there is no CPU fallback on this path.
@@ -24,7 +24,9 @@ EXPORTS = ("dc_abi_version", "dc_last_error",
            "dc_mt19937_seed", "dc_mt19937_advance", "dc_mt19937_table_bytes",
            "dc_mt19937_table_init", "dc_bernoulli_max_draws", "dc_bernoulli_workspace_size",
            "dc_bernoulli", "dc_dropout_apply",
-           "dc_rotary_fwd", "dc_rotary_bwd_workspace_size", "dc_rotary_bwd")
+           "dc_rotary_fwd", "dc_rotary_bwd_workspace_size", "dc_rotary_bwd",
+           "dc_window_fwd_workspace_size", "dc_window_fwd", "dc_window_bwd_workspace_size", "dc_window_bwd",
+           "dc_window_decode_workspace_size", "dc_window_decode")
 
 
 class Desc(ctypes.Structure):
@@ -73,6 +75,14 @@ class RotaryDesc(ctypes.Structure):
                 + [(n, ctypes.c_int64) for n in ("offset", "pos_stride_b", "pos_stride_l")]
                 + [("magnitude", ctypes.c_double), ("eps", ctypes.c_double)]
                 + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "grad_q_stride", "grad_k_stride")])
+
+
+class WindowDesc(ctypes.Structure):
+    """``dc_window_desc``."""
+    _fields_ = ([(n, ctypes.c_int64) for n in ("batch", "heads", "kv_heads", "q_len", "kv_len", "head_dim",
+                                               "offset", "window", "sinks")]
+                + [("dtype", ctypes.c_int32), ("has_scale", ctypes.c_int32), ("scale", ctypes.c_double)]
+                + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "grad_out_stride")])
 
 
 _lib = None
@@ -124,11 +134,20 @@ def lib():
         L.dc_rotary_bwd_workspace_size.argtypes = [RD]
         L.dc_rotary_bwd_workspace_size.restype = SZ
         L.dc_rotary_bwd.argtypes = [RD] + [P] * 13 + [SZ, P]
-        for name in ("dc_rotary_fwd", "dc_rotary_bwd",
+        WD = ctypes.POINTER(WindowDesc)
+        for name in ("dc_window_fwd", "dc_window_bwd", "dc_window_decode"):
+            getattr(L, name + "_workspace_size").argtypes = [WD]
+            getattr(L, name + "_workspace_size").restype = SZ
+        L.dc_window_fwd.argtypes = [WD, P, P, P, P, P, P, SZ, P]
+        L.dc_window_bwd.argtypes = [WD] + [P] * 10 + [SZ, P]
+        L.dc_window_decode.argtypes = [WD, P, P, P, P, ctypes.c_int32, P, P, P, SZ, P]
+        for name in ("dc_window_fwd", "dc_window_bwd", "dc_window_decode", "dc_rotary_fwd", "dc_rotary_bwd",
                      "dc_sdpa_fwd", "dc_sdpa_bwd", "dc_sdpa_decode", "dc_softmax_fwd",
                      "dc_softmax_bwd", "dc_mt19937_advance", "dc_mt19937_table_init",
                      "dc_bernoulli", "dc_dropout_apply",
-           "dc_rotary_fwd", "dc_rotary_bwd_workspace_size", "dc_rotary_bwd"):
+           "dc_rotary_fwd", "dc_rotary_bwd_workspace_size", "dc_rotary_bwd",
+           "dc_window_fwd_workspace_size", "dc_window_fwd", "dc_window_bwd_workspace_size", "dc_window_bwd",
+           "dc_window_decode_workspace_size", "dc_window_decode"):
             getattr(L, name).restype = ctypes.c_int
         _lib = L
     return _lib

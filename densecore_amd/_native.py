@@ -415,6 +415,82 @@ def _rotary_backward(grad_q, grad_k, q, k, inv_freq, positions=None, offset=0, i
     return dq, dk, dwq, dwk
 
 
+def _window_desc(q, k, v, window, sinks, offset, scale, grad_out=None):
+    """Checks the tensors of window attention; returns its descriptor (``dc_window_desc``)."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("window attention takes (B, H, L, E) tensors")
+    B, H, L, E = q.shape
+    Hkv, S = k.shape[1], k.shape[2]
+    if (k.shape != v.shape or k.shape[0] != B or k.shape[3] != E or Hkv == 0 or H % Hkv
+            or (grad_out is not None and grad_out.shape != q.shape)):
+        raise ValueError("window attention q/k/v shapes do not match")
+    if q.device.type != "cuda":
+        raise ValueError("window attention tensors must be on the GPU")
+    if q.dtype not in _DTYPES:
+        raise ValueError("window attention takes float32 or bfloat16 tensors")
+    for t in (k, v, grad_out):
+        if t is not None and (t.device != q.device or t.dtype != q.dtype):
+            raise ValueError("window attention tensors must share one device and dtype")
+    S3 = _lib.ctypes.c_int64 * 3
+    return _lib.WindowDesc(B, H, Hkv, L, S, E, offset, min(window, 2 ** 31), min(sinks, 2 ** 31), _DTYPES[q.dtype],
+                           int(scale is not None), 0.0 if scale is None else scale,
+                           *(S3(*t.stride()[:3]) if t is not None else S3() for t in (q, k, v, grad_out)))
+
+
+def _window_attention(q, k, v, window, sinks=0, offset=0, scale=None):
+    """``dc_window_fwd``: (out, lse)."""
+    q, k, v = _unit_rows(q), _unit_rows(k), _unit_rows(v)
+    d = _window_desc(q, k, v, window, sinks, offset, scale)
+    dev, L_ = q.device, _lib.lib()
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
+    with _on(dev):
+        nbytes = L_.dc_window_fwd_workspace_size(d)
+        ws = _workspace(nbytes, dev) if nbytes else None
+        _lib.check(L_.dc_window_fwd(d, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(ws),
+                                    0 if ws is None else ws.numel(), _stream(dev)))
+    return out, lse
+
+
+def _window_attention_backward(grad_out, q, k, v, out, lse, window, sinks=0, offset=0, scale=None):
+    """``dc_window_bwd``: (dq, dk, dv)."""
+    grad_out, q, k, v = (_unit_rows(t) for t in (grad_out, q, k, v))
+    d = _window_desc(q, k, v, window, sinks, offset, scale, grad_out)
+    dev, L_ = q.device, _lib.lib()
+    if out.shape != q.shape or lse.shape != q.shape[:3] or out.dtype != q.dtype or lse.dtype != torch.float32:
+        raise ValueError("window attention backward shapes do not match")
+    if out.device != dev or lse.device != dev:
+        raise ValueError("window attention tensors must share one device and dtype")
+    out, lse = out.contiguous(), lse.contiguous()
+    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v))
+    with _on(dev):
+        ws = _workspace(L_.dc_window_bwd_workspace_size(d), dev)
+        _lib.check(L_.dc_window_bwd(d, _ptr(grad_out), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq),
+                                    _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream(dev)))
+    return dq, dk, dv
+
+
+def _window_decode(q, k, v, window, sinks=0, lengths=None, scale=None):
+    """``dc_window_decode``: (out, lse) of one query per sequence over the cache."""
+    q, k, v = _unit_rows(q), _unit_rows(k), _unit_rows(v)
+    d = _window_desc(q, k, v, window, sinks, 0, scale)
+    dev, L_ = q.device, _lib.lib()
+    if lengths is not None:
+        if tuple(lengths.shape) != (q.shape[0],) or lengths.dtype not in (torch.int32, torch.int64) \
+                or lengths.device != dev:
+            raise ValueError("window decode lengths must be (B,) int32 or int64 on the tensors' device")
+        lengths = lengths.contiguous()
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
+    with _on(dev):
+        nbytes = L_.dc_window_decode_workspace_size(d)
+        ws = _workspace(nbytes, dev) if nbytes else None
+        _lib.check(L_.dc_window_decode(d, _ptr(q), _ptr(k), _ptr(v), _ptr(lengths),
+                                       0 if lengths is None else lengths.element_size(), _ptr(out), _ptr(lse),
+                                       _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev)))
+    return out, lse
+
+
 def default_scale(head_dim):
     """``sdp::calculate_scale`` as the Python layer passes it (a double)."""
     return 1.0 / math.sqrt(head_dim) if head_dim else 1.0

@@ -1,4 +1,5 @@
-// The C ABI declared in include/dc_attn.h, include/dc_math.h and include/dc_rotary.h: argument checks with the reference's messages,
+// The C ABI declared in include/dc_attn.h, include/dc_math.h, include/dc_rotary.h and
+// include/dc_window.h: argument checks with the reference's messages,
 // scale computation, workspace carving, and dispatch to the kernel launchers.
 //
 // Checks follow the reference boundary (src/lib.rs:555-580 attention_dims, :594-607
@@ -18,8 +19,10 @@
 #include "dc_attn.h"
 #include "dc_math.h"
 #include "dc_rotary.h"
+#include "dc_window.h"
 #include "params.hpp"
 #include "rotary.hpp"
+#include "window.hpp"
 
 namespace dc {
 namespace {
@@ -881,6 +884,174 @@ dc_status dc_rotary_bwd(const dc_rotary_desc *d, const void *grad_q, const void 
     }
     if (a.E == 0) return ok();
     return launched(dc::launch_rotary_norm_bwd(a, d->dtype == DC_BF16, strm));
+}
+
+}  // extern "C"
+
+namespace {
+
+// What the window entries share: sizes, window, scale.
+dc_status check_window(const dc_window_desc *d, int max_head_dim) {
+    if (d == nullptr) return fail(DC_INVALID_ARGUMENT, "window attention descriptor is null");
+    const int64_t dims[6] = {d->batch, d->heads, d->kv_heads, d->q_len, d->kv_len, d->head_dim};
+    for (int64_t x : dims)
+        if (x < 0) return fail(DC_INVALID_ARGUMENT, "window attention takes (B, H, L, E) tensors");
+    if (d->kv_heads <= 0 || d->heads % d->kv_heads != 0)
+        return fail(DC_INVALID_ARGUMENT, "window attention q/k/v shapes do not match");
+    if (d->dtype != DC_F32 && d->dtype != DC_BF16)
+        return fail(DC_INVALID_ARGUMENT, "window attention dtype must be float32 or bfloat16");
+    if (d->window < 1) return fail(DC_INVALID_ARGUMENT, "window attention window must be at least 1");
+    if (d->sinks < 0) return fail(DC_INVALID_ARGUMENT, "window attention sinks must not be negative");
+    if (d->offset < 0) return fail(DC_INVALID_ARGUMENT, "window attention offset must not be negative");
+    if (d->has_scale && !std::isfinite((float)d->scale))
+        return fail(DC_INVALID_ARGUMENT, "window attention scale must be finite");
+    for (int i = 0; i < 3; ++i)
+        if (d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0 || d->grad_out_stride[i] < 0)
+            return fail(DC_INVALID_ARGUMENT, "window attention strides must be non-negative");
+    for (int64_t x : dims)
+        if (x > INT32_MAX / 2) return fail(DC_UNSUPPORTED, "window attention dimension exceeds 2^30");
+    if (d->offset > INT32_MAX / 2) return fail(DC_UNSUPPORTED, "window attention offset exceeds 2^30");
+    if (d->head_dim > max_head_dim)
+        return fail(DC_UNSUPPORTED, "window attention takes head_dim up to " + std::to_string(max_head_dim));
+    return ok();
+}
+
+float window_scale(const dc_window_desc *d) {
+    return d->has_scale ? (float)d->scale : d->head_dim ? (float)(1.0 / std::sqrt((double)d->head_dim)) : 1.f;
+}
+
+// Rows and bases on 16 bytes, whole 16-byte pieces; a tile's row offsets within 32 bits.
+bool window_pieces(const dc_window_desc *d, std::initializer_list<const void *> bases,
+                   std::initializer_list<const int64_t *> strides) {
+    const int64_t per = d->dtype == DC_BF16 ? 8 : 4;
+    bool v = d->head_dim % per == 0;
+    for (const void *p : bases) v = v && aligned16(p);
+    for (const int64_t *s : strides) v = v && s[0] % per == 0 && s[1] % per == 0 && s[2] % per == 0 && s[2] < ((int64_t)1 << 24);
+    return v;
+}
+
+dc_status window_args(const dc_window_desc *d, dc::WinArgs *a) {
+    dc_status st = check_window(d, DC_WINDOW_MAX_HEAD_DIM);
+    if (st != DC_OK) return st;
+    const int64_t rows = (d->q_len + 31) / 32 + 1, keys = (d->kv_len + 31) / 32 + 1;
+    if (d->batch * d->heads > INT32_MAX / 2 || (double)d->batch * d->heads * rows > INT32_MAX / 2 ||
+        (double)d->batch * d->kv_heads * keys > INT32_MAX / 2)
+        return fail(DC_UNSUPPORTED, "window attention has more than 2^30 tiles");
+    *a = dc::WinArgs{};
+    a->B = (int)d->batch, a->H = (int)d->heads, a->Hkv = (int)d->kv_heads;
+    a->L = (int)d->q_len, a->S = (int)d->kv_len, a->E = (int)d->head_dim;
+    a->repeat = a->H / a->Hkv;
+    a->offset = (int)d->offset;
+    a->window = (int)std::min<int64_t>(d->window, INT32_MAX), a->sinks = (int)std::min<int64_t>(d->sinks, INT32_MAX);
+    a->scale = window_scale(d);
+    a->scale_log2 = a->scale * 1.4426950408889634f;
+    for (int i = 0; i < 3; ++i) {
+        a->qs[i] = d->q_stride[i], a->ks[i] = d->k_stride[i], a->vs[i] = d->v_stride[i];
+        a->gs[i] = d->grad_out_stride[i];
+    }
+    a->splits = 1;
+    return ok();
+}
+
+const char *kWindowNull = "window attention got a null pointer for a non-empty tensor";
+
+dc_status window_decode_args(const dc_window_desc *d, dc::WinDecodeArgs *a) {
+    dc_status st = check_window(d, DC_WINDOW_DECODE_MAX_HEAD_DIM);
+    if (st != DC_OK) return st;
+    if (d->q_len != 1) return fail(DC_INVALID_ARGUMENT, "window decode takes q_len == 1");
+    if (d->batch * d->heads > INT32_MAX / 2) return fail(DC_UNSUPPORTED, "window decode batch * heads exceeds 2^30");
+    *a = dc::WinDecodeArgs{};
+    a->B = (int)d->batch, a->H = (int)d->heads, a->Hkv = (int)d->kv_heads, a->S = (int)d->kv_len, a->E = (int)d->head_dim;
+    a->repeat = a->H / a->Hkv;
+    a->window = (int)std::min<int64_t>(d->window, INT32_MAX), a->sinks = (int)std::min<int64_t>(d->sinks, INT32_MAX);
+    a->scale_log2 = window_scale(d) * 1.4426950408889634f;
+    for (int i = 0; i < 3; ++i) a->qs[i] = d->q_stride[i], a->ks[i] = d->k_stride[i], a->vs[i] = d->v_stride[i];
+    a->splits = dc::window_decode_splits(*a, d->dtype == DC_BF16);
+    return ok();
+}
+
+size_t window_decode_ws(const dc::WinDecodeArgs &a) {
+    return a.splits > 1 ? round_up((size_t)a.B * a.H * a.splits * (a.E + 2) * sizeof(float)) : 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dc_window_fwd_workspace_size(const dc_window_desc *d) {
+    dc::WinArgs a;
+    if (window_args(d, &a) != DC_OK) return 0;
+    return round_up(dc::window_fwd_part_bytes(a, d->dtype == DC_BF16));
+}
+
+dc_status dc_window_fwd(const dc_window_desc *d, const void *q, const void *k, const void *v, void *out,
+                        float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+    dc::WinArgs a;
+    dc_status st = window_args(d, &a);
+    if (st != DC_OK) return st;
+    const int64_t nq = (int64_t)a.B * a.H * a.L, nkv = (int64_t)a.B * a.Hkv * a.S * a.E;
+    if (nq == 0) return ok();
+    if (!present(q, nq * a.E) || !present(k, nkv) || !present(v, nkv) || !present(out, nq * a.E) || lse == nullptr)
+        return fail(DC_INVALID_ARGUMENT, kWindowNull);
+    a.q = q, a.k = k, a.v = v, a.out = out, a.lse = lse;
+    a.vec = window_pieces(d, {q, k, v, out}, {a.qs, a.ks, a.vs});
+    a.part = static_cast<float *>(workspace);
+    return launched(dc::launch_window_fwd(a, d->dtype == DC_BF16, workspace_bytes, static_cast<hipStream_t>(stream)));
+}
+
+size_t dc_window_bwd_workspace_size(const dc_window_desc *d) {
+    dc::WinArgs a;
+    if (window_args(d, &a) != DC_OK) return 0;
+    return round_up((size_t)a.B * a.H * a.L * sizeof(float));
+}
+
+dc_status dc_window_bwd(const dc_window_desc *d, const void *grad_out, const void *q, const void *k,
+                        const void *v, const void *out, const float *lse, void *dq, void *dk, void *dv,
+                        void *workspace, size_t workspace_bytes, void *stream) {
+    dc::WinArgs a;
+    dc_status st = window_args(d, &a);
+    if (st != DC_OK) return st;
+    const int64_t nq = (int64_t)a.B * a.H * a.L, nkv = (int64_t)a.B * a.Hkv * a.S * a.E;
+    if (!present(grad_out, nq * a.E) || !present(q, nq * a.E) || !present(k, nkv) || !present(v, nkv) ||
+        !present(out, nq * a.E) || !present(lse, nq) || !present(dq, nq * a.E) || !present(dk, nkv) ||
+        !present(dv, nkv))
+        return fail(DC_INVALID_ARGUMENT, kWindowNull);
+    if (a.E == 0 || a.B == 0 || a.H == 0 || (a.L == 0 && a.S == 0)) return ok();
+    if (nq > 0 && (workspace == nullptr || workspace_bytes < dc_window_bwd_workspace_size(d)))
+        return fail(DC_INVALID_ARGUMENT, "window attention backward workspace is too small");
+    a.dout = grad_out, a.q = q, a.k = k, a.v = v, a.out_in = out, a.lse_in = lse;
+    a.dq = dq, a.dk = dk, a.dv = dv;
+    a.dsum = static_cast<float *>(workspace);
+    a.vec = window_pieces(d, {grad_out, q, k, v, out, dq, dk, dv}, {a.qs, a.ks, a.vs, a.gs});
+    return launched(dc::launch_window_bwd(a, d->dtype == DC_BF16, static_cast<hipStream_t>(stream)));
+}
+
+size_t dc_window_decode_workspace_size(const dc_window_desc *d) {
+    dc::WinDecodeArgs a;
+    if (window_decode_args(d, &a) != DC_OK) return 0;
+    return window_decode_ws(a);
+}
+
+dc_status dc_window_decode(const dc_window_desc *d, const void *q, const void *k, const void *v,
+                           const void *lengths, int32_t length_bytes, void *out, float *lse, void *workspace,
+                           size_t workspace_bytes, void *stream) {
+    dc::WinDecodeArgs a;
+    dc_status st = window_decode_args(d, &a);
+    if (st != DC_OK) return st;
+    if (length_bytes != 0 && length_bytes != 4 && length_bytes != 8)
+        return fail(DC_INVALID_ARGUMENT, "window decode lengths must be int32 or int64");
+    const int64_t nq = (int64_t)a.B * a.H, nkv = (int64_t)a.B * a.Hkv * a.S * a.E;
+    if (nq == 0) return ok();
+    if (!present(q, nq * a.E) || !present(k, nkv) || !present(v, nkv) || !present(out, nq * a.E) || lse == nullptr ||
+        (length_bytes != 0 && lengths == nullptr))
+        return fail(DC_INVALID_ARGUMENT, kWindowNull);
+    if (window_decode_ws(a) > 0 && (workspace == nullptr || workspace_bytes < window_decode_ws(a)))
+        return fail(DC_INVALID_ARGUMENT, "window decode workspace is too small");
+    if ((double)a.B * a.H * a.splits > INT32_MAX / 2) return fail(DC_UNSUPPORTED, "window decode has more than 2^30 pieces");
+    a.q = q, a.k = k, a.v = v, a.lengths = lengths, a.length_bytes = length_bytes, a.out = out, a.lse = lse;
+    a.part = static_cast<float *>(workspace);
+    a.vec = window_pieces(d, {q, k, v}, {a.qs, a.ks, a.vs});
+    return launched(dc::launch_window_decode(a, d->dtype == DC_BF16, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

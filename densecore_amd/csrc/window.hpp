@@ -1,0 +1,274 @@
+// Attention with a sliding window and sinks (dc_window.h): parameter block, launchers, and what the
+// forward and backward kernels share: which key tiles a block of queries reads, operand fragments of
+// both types and tiles of rows in LDS.
+//
+// One source for both types.  bf16 operands enter the MFMAs as they are, and what the kernels compute
+// (P, dS) as two bf16 terms hi + lo, carried to 2^-17.  float32 operands are split exactly into three
+// bf16 parts (x3.hpp), six products each, error below the float32 MFMA's.  So neither type has a
+// rounding to fewer bits before the result's own.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "common.hpp"
+#include "tile_bf16.hpp"
+#include "x3.hpp"
+
+namespace dc {
+
+struct WinArgs {
+    int B, H, Hkv, L, S, E, repeat;
+    int offset, window, sinks;
+    float scale, scale_log2;  // natural and base 2
+    const void *q, *k, *v, *dout, *out_in;
+    const float *lse_in;
+    int64_t qs[3], ks[3], vs[3], gs[3];  // strides: batch, head, row
+    void *out;
+    float *lse;
+    void *dq, *dk, *dv;
+    float *dsum;          // (B, H, L): rowsum(dO * O)
+    bool pack;            // forward: rows of all the heads of a kv head share tiles
+    int splits;           // forward: pieces of each tile's keys
+    float *part, *part_lse;
+    bool vec;             // 16-byte pieces: rows and bases on 16 bytes, E a whole number of pieces
+};
+
+hipError_t launch_window_fwd(const WinArgs &a, bool bf16, size_t part_bytes, hipStream_t st);
+size_t window_fwd_part_bytes(const WinArgs &a, bool bf16);
+hipError_t launch_window_bwd(const WinArgs &a, bool bf16, hipStream_t st);
+
+struct WinDecodeArgs {
+    int B, H, Hkv, S, E, repeat;
+    int window, sinks;
+    float scale_log2;
+    const void *q, *k, *v, *lengths;
+    int length_bytes;
+    int64_t qs[3], ks[3], vs[3];
+    void *out;
+    float *lse;
+    float *part;
+    int splits;
+    bool vec;
+};
+hipError_t launch_window_decode(const WinDecodeArgs &a, bool bf16, hipStream_t st);
+int window_decode_splits(const WinDecodeArgs &a, bool bf16);
+
+namespace {
+
+// Whether the query at position p sees key s (s < S is the caller's).
+DEVI bool sees(int p, int s, int window, int sinks) { return s <= p && (p - s < window || s < sinks); }
+
+// The key tiles (of BN keys) that queries at positions p0 .. p1 read: ns tiles from key 0 (sinks), then
+// those from tile tb; n in all.  One run from tile 0 where the two meet.
+struct Band {
+    int ns, tb, n;
+    __host__ __device__ int tile(int i) const { return i < ns ? i : tb + (i - ns); }
+};
+__host__ __device__ inline Band band_of(int p0, int p1, int S, int window, int sinks, int BN) {
+    const int hi = p1 < S - 1 ? p1 + 1 : S;           // keys below hi
+    const int lo = p0 >= window ? p0 - window + 1 : 0;  // and from lo on, or below sinks
+    const int sink_end = sinks < hi ? sinks : hi;
+    Band b;
+    b.ns = (sink_end + BN - 1) / BN;
+    b.tb = lo / BN;
+    int te = lo < hi ? (hi + BN - 1) / BN : b.tb;
+    if (b.ns > 0 && b.ns >= b.tb) {  // meet: one run
+        if (te < b.ns) te = b.ns;
+        b.ns = 0, b.tb = 0;
+    }
+    b.n = b.ns + (te - b.tb);
+    return b;
+}
+
+// Operands of one type.
+template <typename T>
+struct Ops;
+template <>
+struct Ops<__bf16> {
+    typedef bf16x8 Frag;
+    struct PFrag {
+        bf16x8 h, l;
+    };
+    template <int R, int D>
+    struct Tile {
+        u32x4 p[CMTile<R, D>::SLOTS];
+    };
+    template <int R, int D>
+    DEVI static Frag row(const Tile<R, D> &t, uint32_t base, int row0, int st) { return row_frag<R, D>(t.p, base, row0, st); }
+    template <int R, int D>
+    DEVI static Frag tr(const Tile<R, D> &t, uint32_t base, int row0, int dt) { return tr_frag<R, D>(t.p, base, row0, dt); }
+    DEVI static f32x16 mma(Frag a, Frag b, f32x16 c) { return mfma_bf16(a, b, c); }
+    DEVI static PFrag split(const f32x16 &x, int at) {
+        PFrag p;
+        split_bf16(x, at, p.h, p.l);
+        return p;
+    }
+    DEVI static f32x16 mma_p(Frag a, const PFrag &p, f32x16 c) { return mfma_bf16(a, p.h, mfma_bf16(a, p.l, c)); }
+    // Dims d0 .. d0 + 7 of a row (0 past E, and all 0 without `in`).
+    template <bool VEC>
+    DEVI static Frag load(const __bf16 *row, int d0, int E, bool in) {
+        Frag f;
+        if (VEC) {
+            const u32x4 z = {0u, 0u, 0u, 0u};
+            f = __builtin_bit_cast(bf16x8, in && d0 < E ? *reinterpret_cast<const u32x4 *>(row + d0) : z);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = in && d0 + e < E ? row[d0 + e] : static_cast<__bf16>(0.f);
+        }
+        return f;
+    }
+    DEVI static Frag neg(Frag f) {
+        u32x4 x = __builtin_bit_cast(u32x4, f);
+        x ^= 0x80008000u;
+        return __builtin_bit_cast(bf16x8, x);
+    }
+    // a . b of two fragments' own 8 dims.
+    DEVI static float dot(Frag a, Frag b) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(bf16_to_f32(a[e]), bf16_to_f32(b[e]), s);
+        return s;
+    }
+};
+template <>
+struct Ops<float> {
+    typedef X3 Frag;
+    typedef X3 PFrag;
+    template <int R, int D>
+    using Tile = X3Tile<R, D>;
+    template <int R, int D>
+    DEVI static Frag row(const Tile<R, D> &t, uint32_t base, int row0, int st) { return row_frag_x3<R, D>(t, base, row0, st); }
+    template <int R, int D>
+    DEVI static Frag tr(const Tile<R, D> &t, uint32_t base, int row0, int dt) { return tr_frag_x3<R, D>(t, base, row0, dt); }
+    DEVI static f32x16 mma(const Frag &a, const Frag &b, f32x16 c) { return mfma_x3(a, b, c); }
+    DEVI static PFrag split(const f32x16 &x, int at) { return split3(x, at); }
+    DEVI static f32x16 mma_p(const Frag &a, const PFrag &p, f32x16 c) { return mfma_x3(a, p, c); }
+    template <bool VEC>
+    DEVI static Frag load(const float *row, int d0, int E, bool in) {
+        f32x4 x[2];
+        load_chunk<VEC>(x, row, d0, in ? E : 0);
+        return split_chunk(x);
+    }
+    DEVI static Frag neg(const Frag &f) { return {Ops<__bf16>::neg(f.h), Ops<__bf16>::neg(f.m), Ops<__bf16>::neg(f.l)}; }
+    DEVI static float dot(const Frag &a, const Frag &b) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            s = fmaf((bf16_to_f32(a.l[e]) + bf16_to_f32(a.m[e])) + bf16_to_f32(a.h[e]),
+                     (bf16_to_f32(b.l[e]) + bf16_to_f32(b.m[e])) + bf16_to_f32(b.h[e]), s);
+        return s;
+    }
+};
+
+// R rows of D dims on their way from memory (row stride `ld`) into an LDS tile by THREADS threads: start()
+// issues the loads, finish() ends them (the caller then synchronizes).  Rows from `rows` on and dims
+// past E are 0.
+//
+// bf16 in 16-byte pieces: global_load_lds, lane l taking row l of a 64-row block, no registers between.
+// Dims past E are zeroed once for the kernel's life by clear() (no transfer writes there).  Otherwise,
+// and float32 (split on the way), through registers.
+template <typename T, int R, int D, int THREADS, bool VEC>
+struct Stage;
+template <int R, int D, int THREADS>
+struct Stage<__bf16, R, D, THREADS, true> {
+    typedef Ops<__bf16>::Tile<R, D> Tile;
+    DEVI static void clear(Tile &t, int E, int tid) {
+        for (int i = (E / 8) * CMTile<R, D>::P + tid; i < CMTile<R, D>::SLOTS; i += THREADS) t.p[i] = u32x4{0u, 0u, 0u, 0u};
+    }
+    DEVI void start(Tile &t, const __bf16 *src, int64_t ld, int rows, int E, int tid) {
+        static_assert(R % 64 == 0 || R == 32, "64 rows at a time, or half a wave's");
+        constexpr int W = THREADS / 64, RB = R / 64 ? R / 64 : 1, NT = CMTile<R, D>::C * RB, count = (NT + W - 1) / W;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+        const uint32_t loff = (uint32_t)lane * (uint32_t)(ld * 2);
+#pragma unroll
+        for (int j = 0; j < count; ++j) {
+            const int inst = wave + W * j, c = inst / RB, rb = inst % RB;
+            if (inst >= NT || 8 * c >= E) continue;  // wave-uniform
+            u32x4 *d = t.p + c * CMTile<R, D>::P + 64 * rb;
+            const __bf16 *s = src + (int64_t)(64 * rb) * ld + 8 * c;
+            const int row = 64 * rb + lane;
+            if (R >= 64 && rows >= R) {
+                lds_dma16_off(s, loff, d);
+            } else if (row < R) {
+                if (row < rows) lds_dma16_off(s, loff, d);
+                else d[lane] = u32x4{0u, 0u, 0u, 0u};
+            }
+        }
+    }
+    DEVI void finish(Tile &, int) { wait_vmem(); }
+};
+template <int R, int D, int THREADS>
+struct Stage<__bf16, R, D, THREADS, false> {
+    typedef Ops<__bf16>::Tile<R, D> Tile;
+    static constexpr int C = D / 8, N = (R * C + THREADS - 1) / THREADS;
+    bf16x8 x[N];
+    DEVI static void clear(Tile &, int, int) {}
+    DEVI void start(Tile &, const __bf16 *src, int64_t ld, int rows, int E, int tid) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = tid + THREADS * j, r = i / C, c = i % C;
+            x[j] = Ops<__bf16>::load<false>(src + (int64_t)min(r, rows - 1) * ld, 8 * c, E, r < rows);
+        }
+    }
+    DEVI void finish(Tile &t, int tid) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = tid + THREADS * j, r = i / C, c = i % C;
+            if (i < R * C) t.p[c * CMTile<R, D>::P + r] = __builtin_bit_cast(u32x4, x[j]);
+        }
+    }
+};
+template <int R, int D, int THREADS, bool VEC>
+struct Stage<float, R, D, THREADS, VEC> {
+    typedef Ops<float>::Tile<R, D> Tile;
+    typedef X3Stage<R, D, THREADS, VEC> X;
+    X s;
+    DEVI static void clear(Tile &, int, int) {}
+    DEVI void start(Tile &, const float *src, int64_t ld, int rows, int E, int tid) {
+#pragma unroll
+        for (int j = 0; j < X::N; ++j) {
+            int r, c;
+            X::place(j, tid, r, c);
+            if (X::TOTAL % THREADS != 0 && tid + THREADS * j >= X::TOTAL) return;
+            load_chunk<VEC>(s.x[j], src + (int64_t)min(r, rows - 1) * ld, 8 * c, r < rows ? E : 0);
+        }
+    }
+    DEVI void finish(Tile &t, int tid) { s.store(t, tid); }
+};
+
+// Four consecutive dims of a row of a result.
+template <typename T, bool VEC>
+DEVI void store4(T *row, int d, int E, float x0, float x1, float x2, float x3) {
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    if (VEC) {
+        if (d < E) *reinterpret_cast<vec4 *>(row + d) = vec4{from_f32<T>(x0), from_f32<T>(x1), from_f32<T>(x2), from_f32<T>(x3)};
+    } else {
+        const float x[4] = {x0, x1, x2, x3};
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (d + u < E) row[d + u] = from_f32<T>(x[u]);
+    }
+}
+
+// a . b over E dims in plain float32, for rows computed again.
+template <typename T>
+DEVI float plain_dot(const T *a, const T *b, int E) {
+    float s = 0.f;
+    for (int d = 0; d < E; ++d) s = fmaf(to_f32<T>(a[d]), to_f32<T>(b[d]), s);
+    return s;
+}
+
+DEVI float wave_max(float x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+    return x;
+}
+DEVI float wave_sum(float x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+    return x;
+}
+
+}  // namespace
+}  // namespace dc

@@ -1,0 +1,335 @@
+// Forward of attention with a sliding window and sinks (window.hpp): out = softmax over the visible
+// keys of scale q k^T, times v, in one pass with a running maximum and sum.
+//
+// A workgroup of 4 waves owns 128 rows (queries) and visits only the key tiles one of them sees
+// (Band): its window's and the sinks'.  A wave owns 32 rows, held in registers as the second operand of
+// S^T = K Q^T, so a lane holds one row's softmax state; P goes straight from S^T's accumulators into
+// O^T += V^T P^T.  K and V tiles are double-buffered in LDS.  Rows of short queries (a few tokens of
+// each head that shares a kv head) are packed into one tile.
+//
+// Where a result is not finite (an infinite or NaN operand, which matrix products spread to rows
+// that do not see it) the row is computed again in plain float32 over its visible keys alone.
+#include <algorithm>
+
+#include "params.hpp"
+#include "window.hpp"
+
+namespace dc {
+namespace {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kM = 32 * kWaves;
+template <typename T>
+constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // keys per tile
+template <typename T, int D>
+constexpr int kWavesPerSimd = sizeof(T) == 2 || D <= 64 ? 2 : 1;  // LDS: 110 KB of float32 tiles at D = 128
+
+// Row r of a group of `pack`ed heads (or of one head) as (head within the group, query).
+struct RowAt {
+    int h, l;
+};
+DEVI RowAt row_at(const WinArgs &a, int r) { return a.pack ? RowAt{r / a.L, r % a.L} : RowAt{0, r}; }
+// The first and last position of rows r0 .. r1.
+DEVI void positions(const WinArgs &a, int r0, int r1, int &p0, int &p1) {
+    if (a.pack && r0 / a.L != r1 / a.L) {
+        p0 = a.offset, p1 = a.offset + a.L - 1;
+    } else {
+        p0 = a.offset + row_at(a, r0).l, p1 = a.offset + row_at(a, r1).l;
+    }
+}
+
+// One row again, keys of tiles [i0, i1): lanes are keys for the scores and dims for the output
+// (dims lane and lane + 64).  The maximum and sum first, so that the output is a sum of P / sum times v and
+// does not overflow where the result does not.
+template <typename T>
+DEVI void plain_row(const WinArgs &a, const T *q, const T *kb, const T *vb, int p, Band band, int i0, int i1, int lane,
+                    float (&o)[2], float &m, float &sum) {
+    constexpr int BN = kKeys<T>;
+    auto score = [&](int n0, bool &ok) {
+        const int key = n0 + lane;
+        ok = lane < BN && key < a.S && sees(p, key, a.window, a.sinks);
+        return ok ? plain_dot<T>(q, kb + key * a.ks[2], a.E) * a.scale_log2 : -INFINITY;
+    };
+    o[0] = o[1] = sum = 0.f, m = -INFINITY;
+    bool ok;
+    for (int i = i0; i < i1; ++i) {
+        const float s = score(band.tile(i) * BN, ok);
+        const float top = fmaxf(m, wave_max(s)), base = top == -INFINITY ? 0.f : top;
+        sum = sum * exp2_fast(m - base) + wave_sum(ok ? exp2_fast(s - base) : 0.f);
+        m = top;
+    }
+    const float base = m == -INFINITY ? 0.f : m, inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int i = i0; i < i1; ++i) {
+        const int n0 = band.tile(i) * BN;
+        const float s = score(n0, ok), pr = ok ? exp2_fast(s - base) * inv : 0.f;
+        for (uint64_t left = __ballot(ok); left; left &= left - 1) {
+            const int j = __builtin_ctzll(left);
+            const float pj = __shfl(pr, j, 64);
+            const T *v = vb + (n0 + j) * a.vs[2];
+            if (lane < a.E) o[0] = fmaf(pj, to_f32<T>(v[lane]), o[0]);
+            if (lane + 64 < a.E) o[1] = fmaf(pj, to_f32<T>(v[lane + 64]), o[1]);
+        }
+    }
+}
+
+template <typename T, int D, bool VEC>
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) void window_fwd_kernel(WinArgs a) {
+    typedef Ops<T> O;
+    constexpr int BN = kKeys<T>, NT = BN / 32, KSTEP = D / 16, NDT = D / 32;
+    typedef Stage<T, BN, D, kThreads, VEC> St;
+    __shared__ typename St::Tile sk[2], sv[2];
+
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int G = a.pack ? a.repeat : 1, rows = G * a.L, groups = a.H / G;
+    const int nqt = (rows + kM - 1) / kM;
+    int w = logical_block();
+    const int piece = w % a.splits;
+    w /= a.splits;
+    const int qt = nqt - 1 - w % nqt, grp = w / nqt;
+    const int b = grp / groups, h0 = grp % groups * G, hk = h0 / a.repeat;
+    const int r0 = qt * kM, wr0 = r0 + 32 * wave, r = wr0 + lr;
+    const bool in = r < rows;
+    const RowAt at = row_at(a, in ? r : rows - 1);
+    const int p = in ? a.offset + at.l : -1;  // -1: sees nothing
+    const int64_t row = ((int64_t)b * a.H + h0 + at.h) * a.L + at.l;  // of out and lse
+
+    int p0, p1, wp0 = 0, wp1 = -1;  // positions of the workgroup's rows and of the wave's (none: empty)
+    positions(a, r0, min(r0 + kM, rows) - 1, p0, p1);
+    if (wr0 < rows) positions(a, wr0, min(wr0 + 32, rows) - 1, wp0, wp1);
+    const Band band = band_of(p0, p1, a.S, a.window, a.sinks, BN);
+    const int i0 = (int)((int64_t)piece * band.n / a.splits), i1 = (int)((int64_t)(piece + 1) * band.n / a.splits);
+
+    const T *kb = static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[1];
+    const T *vb = static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1];
+    const T *q = static_cast<const T *>(a.q) + b * a.qs[0] + (h0 + at.h) * a.qs[1] + at.l * a.qs[2];
+
+    // Scores are fma(q.k, c, -m) in base 2; a negative scale is a sign flip of the queries, and a zero
+    // one the smallest normal number (every visible key then gets P = 1).
+    const float c = fmaxf(fabsf(a.scale_log2), 0x1p-126f);
+    typename O::Frag qf[KSTEP];
+#pragma unroll
+    for (int t = 0; t < KSTEP; ++t) {
+        qf[t] = O::template load<VEC>(q, 16 * t + 8 * g, a.E, in);
+        if (a.scale_log2 < 0.f) qf[t] = O::neg(qf[t]);
+    }
+    f32x16 acc[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
+    float m_run = -INFINITY, l_part = 0.f;  // l_part: this half-wave's keys only
+
+    const uint32_t rowb = row_lanebase<BN, D>(lane), trb = tr_lanebase<BN, D>(lane);
+    St kst, vst;
+    auto start = [&](int i) {
+        const int n0 = band.tile(i) * BN, nr = min(BN, a.S - n0), buf = (i - i0) & 1;
+        kst.start(sk[buf], kb + (int64_t)n0 * a.ks[2], a.ks[2], nr, a.E, tid);
+        vst.start(sv[buf], vb + (int64_t)n0 * a.vs[2], a.vs[2], nr, a.E, tid);
+    };
+    auto finish = [&](int i) {
+        kst.finish(sk[(i - i0) & 1], tid);
+        vst.finish(sv[(i - i0) & 1], tid);
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) St::clear(sk[i], a.E, tid), St::clear(sv[i], a.E, tid);
+    if (i0 < i1) start(i0), finish(i0);
+
+    auto step = [&](int i) {
+        const int n0 = band.tile(i) * BN, buf = (i - i0) & 1;
+        bool live[NT], any = false;
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt) {
+            const int k0 = n0 + 32 * kt;
+            live[kt] = k0 < a.S && k0 <= wp1 && (wp0 - (k0 + 31) < a.window || k0 < a.sinks);
+            any |= live[kt];
+        }
+        if (!any) return;
+        f32x16 s[NT];
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[kt][e] = 0.f;
+            if (!live[kt]) continue;
+#pragma unroll
+            for (int st = 0; st < KSTEP; ++st) s[kt] = O::mma(O::row(sk[buf], rowb, 32 * kt, st), qf[st], s[kt]);
+        }
+        const bool all = n0 + BN <= a.S && n0 + BN - 1 <= wp0 && (wp1 - n0 < a.window || n0 + BN <= a.sinks);
+        if (!all) {
+#pragma unroll
+            for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = n0 + 32 * kt + acc_row(e, g);
+                    if (!live[kt] || key >= a.S || !sees(p, key, a.window, a.sinks)) s[kt][e] = -INFINITY;
+                }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kt][e]);
+        mx = xor32_max(mx) * c;
+        // The reference of the exponents moves only when some row's maximum exceeds it by more than 8.
+        if (__any(mx > m_run + 8.f)) {
+            const float m_new = fmaxf(m_run, mx);
+            const float alpha = exp2_fast(m_run - (m_new == -INFINITY ? 0.f : m_new));
+            l_part *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[dt][e] *= alpha;
+            m_run = m_new;
+        }
+        const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[kt][e] = exp2_fast(fmaf(s[kt][e], c, neg_m));
+                l_part += s[kt][e];
+            }
+            if (!live[kt]) continue;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const typename O::PFrag pf = O::split(s[kt], 8 * u);
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) acc[dt] = O::mma_p(O::tr(sv[buf], trb, 32 * kt + 16 * u, dt), pf, acc[dt]);
+            }
+        }
+    };
+    for (int i = i0; i < i1; ++i) {
+        __syncthreads();  // tile i is there, and everyone is done with tile i - 1
+        if (i + 1 < i1) start(i + 1);
+        step(i);
+        if (i + 1 < i1) finish(i + 1);
+    }
+
+    const float l_run = xor32_add(l_part);
+    const bool empty = l_run == 0.f;
+    const float inv = empty ? 0.f : 1.f / l_run;
+    float test = l_run * 0.f;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) test += not_finite(acc[dt]);
+    const uint64_t wrong = __ballot(in && test != 0.f);
+    uint32_t again = (uint32_t)wrong | (uint32_t)(wrong >> 32);
+    const int64_t nrows = (int64_t)a.B * a.H * a.L;
+    if (in && !((again >> lr) & 1)) {
+        const float lse = (m_run + log2_fast(l_run)) * kLn2;
+        if (a.splits > 1) {
+            const int64_t slot = piece * nrows + row;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    store4<float, VEC>(a.part + slot * a.E, dt * 32 + acc_row(e, g), a.E, acc[dt][e] * inv, acc[dt][e + 1] * inv,
+                                       acc[dt][e + 2] * inv, acc[dt][e + 3] * inv);
+            if (g == 0) a.part_lse[slot] = empty ? -INFINITY : lse;
+        } else {
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    store4<T, VEC>(static_cast<T *>(a.out) + row * a.E, dt * 32 + acc_row(e, g), a.E, acc[dt][e] * inv,
+                                   acc[dt][e + 1] * inv, acc[dt][e + 2] * inv, acc[dt][e + 3] * inv);
+            if (g == 0) a.lse[row] = empty ? 0.f : lse;
+        }
+    }
+    for (; again; again &= again - 1) {
+        const int rr = wr0 + __builtin_ctz(again);
+        const RowAt ra = row_at(a, rr);
+        const int64_t orow = ((int64_t)b * a.H + h0 + ra.h) * a.L + ra.l;
+        float o[2], m, sum;
+        plain_row<T>(a, static_cast<const T *>(a.q) + b * a.qs[0] + (h0 + ra.h) * a.qs[1] + ra.l * a.qs[2], kb, vb,
+                     a.offset + ra.l, band, i0, i1, lane, o, m, sum);
+        const bool none = sum == 0.f;
+        const float lse = (m + log2_fast(sum)) * kLn2;
+        const int64_t slot = piece * nrows + orow;
+#pragma unroll
+        for (int d = lane, j = 0; j < 2; ++j, d += 64) {
+            if (d >= a.E) continue;
+            if (a.splits > 1) a.part[slot * a.E + d] = o[j];
+            else static_cast<T *>(a.out)[orow * a.E + d] = from_f32<T>(o[j]);
+        }
+        if (lane == 0) {
+            if (a.splits > 1) a.part_lse[slot] = none ? -INFINITY : lse;
+            else a.lse[orow] = none ? 0.f : lse;
+        }
+    }
+}
+
+// Joins the pieces of each row, 16 lanes per row: lse = log sum exp(lse_i), out = sum exp(lse_i - lse) o_i.
+template <typename T>
+__global__ __launch_bounds__(256) void window_merge_kernel(WinArgs a) {
+    const int64_t nrows = (int64_t)a.B * a.H * a.L, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (row >= nrows) return;
+    const int part = threadIdx.x & 15;
+    float top = -INFINITY, sum = 0.f;
+    for (int i = 0; i < a.splits; ++i) top = fmaxf(top, a.part_lse[i * nrows + row]);
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int i = 0; i < a.splits; ++i) sum += exp2_fast((a.part_lse[i * nrows + row] - base) * kLog2e);
+    const bool empty = sum == 0.f;
+    const float inv = empty ? 0.f : 1.f / sum;
+    for (int d = part; d < a.E; d += 16) {
+        float o = 0.f;
+        for (int i = 0; i < a.splits; ++i)
+            o = fmaf(exp2_fast((a.part_lse[i * nrows + row] - base) * kLog2e) * inv, a.part[(i * nrows + row) * a.E + d], o);
+        static_cast<T *>(a.out)[row * a.E + d] = from_f32<T>(o);
+    }
+    if (part == 0) a.lse[row] = empty ? 0.f : base + log2_fast(sum) * kLn2;
+}
+
+// Heads that share a kv head share tiles where a head's queries fill less than half of one.
+bool packs(const WinArgs &a) { return a.repeat > 1 && a.L <= kM / 2; }
+
+int64_t blocks_of(const WinArgs &a, bool pack) {
+    const int64_t rows = (int64_t)(pack ? a.repeat : 1) * a.L;
+    return (rows + kM - 1) / kM * a.B * (a.H / (pack ? a.repeat : 1));
+}
+
+// Pieces of each tile's keys: where the tiles fill at most half of the CUs, as many as fill them, of at
+// least 256 keys.
+int plan_splits(const WinArgs &a, bool bf16) {
+    const int64_t blocks = blocks_of(a, packs(a)), cus = device_cus();
+    if (blocks == 0 || cus <= 0 || 2 * blocks > cus) return 1;
+    const int BN = bf16 ? kKeys<__bf16> : kKeys<float>;
+    const int64_t span = std::min<int64_t>(a.S, (int64_t)a.window + a.sinks + std::min(a.L, kM));
+    const int64_t most = std::max<int64_t>(1, span / std::max(256, BN));
+    return (int)std::min(most, cus / blocks);
+}
+
+template <typename T, int D, bool VEC>
+hipError_t launch_v(const WinArgs &a, hipStream_t st) {
+    return_if(launch(window_fwd_kernel<T, D, VEC>, dim3((unsigned)(blocks_of(a, a.pack) * a.splits)), dim3(kThreads), st, a));
+    if (a.splits == 1) return hipSuccess;
+    const int64_t nrows = (int64_t)a.B * a.H * a.L;
+    return launch(window_merge_kernel<T>, dim3((unsigned)((nrows + 15) / 16)), dim3(256), st, a);
+}
+template <typename T, int D>
+hipError_t launch_d(const WinArgs &a, hipStream_t st) {
+    return a.vec ? launch_v<T, D, true>(a, st) : launch_v<T, D, false>(a, st);
+}
+template <typename T>
+hipError_t launch_t(const WinArgs &a, hipStream_t st) {
+    if (a.E <= 32) return launch_d<T, 32>(a, st);
+    if (a.E <= 64) return launch_d<T, 64>(a, st);
+    return launch_d<T, 128>(a, st);
+}
+
+}  // namespace
+
+size_t window_fwd_part_bytes(const WinArgs &a, bool bf16) {
+    const int n = plan_splits(a, bf16);
+    return n > 1 ? (size_t)n * a.B * a.H * a.L * (a.E + 1) * sizeof(float) : 0;
+}
+
+hipError_t launch_window_fwd(const WinArgs &args, bool bf16, size_t part_bytes, hipStream_t st) {
+    WinArgs a = args;
+    a.pack = packs(a);
+    a.splits = plan_splits(a, bf16);
+    if (a.splits > 1 && (!a.part || part_bytes < window_fwd_part_bytes(a, bf16))) a.splits = 1;
+    if (a.splits > 1) a.part_lse = a.part + (size_t)a.splits * a.B * a.H * a.L * a.E;
+    return bf16 ? launch_t<__bf16>(a, st) : launch_t<float>(a, st);
+}
+
+}  // namespace dc

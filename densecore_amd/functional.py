@@ -289,6 +289,63 @@ def flash_decode(query, key, value, scale=None):
     return _native._flash_decode(query, key, value, None if scale is None else float(scale))[0]
 
 
+def _window_numbers(window, sinks, offset, scale):
+    for name, n, least in (("window", window, 1), ("sinks", sinks, 0), ("offset", offset, 0)):
+        if isinstance(n, (bool, np.bool_)) or not isinstance(n, numbers.Integral):
+            raise TypeError(f"window attention {name} must be an int")
+        if n < least:
+            raise ValueError(f"window attention {name} must be at least {least}")
+    if scale is not None:
+        if isinstance(scale, (bool, np.bool_)) or not isinstance(scale, numbers.Real):
+            raise TypeError("scale must be real")
+        scale = float(scale)
+        if not math.isfinite(scale):
+            raise ValueError("window attention scale must be finite")
+    return int(window), int(sinks), int(offset), scale
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, offset, scale):
+        out, lse = _native._window_attention(q, k, v, window, sinks, offset, scale)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.args = (window, sinks, offset, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return (*_native._window_attention_backward(grad, *ctx.saved_tensors, *ctx.args), None, None, None, None)
+
+
+def window_attention(query, key, value, window, sinks=0, offset=0, scale=None):
+    """Causal attention in which a query sees the last ``window`` keys, its own among them, and the first
+    ``sinks`` ones: query (B, H, L, E) over key and value (B, Hkv, S, E), H a multiple of Hkv.
+
+    The query in row l stands at position ``offset + l`` and key s at position s: key s is visible iff
+    ``s <= p and (s > p - window or s < sinks)`` (``offset`` 0 is the alignment of ``is_causal``; the next
+    L tokens of a sequence of S have ``offset = S - L``).  The work is that of the visible pairs, no mask
+    is formed, and keys that are not visible have no influence, whatever they hold.  A query that sees no
+    key gives 0 and no gradients.  Float32 or bf16, head dims up to 128, any strides; gradients are
+    identical from run to run.  No counterpart in the reference."""
+    _check_tensors("attention", query=query, key=key, value=value)
+    args = _window_numbers(window, sinks, offset, scale)
+    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+        return _WindowAttention.apply(query, key, value, *args)
+    return _native._window_attention(query, key, value, *args)[0]
+
+
+def window_decode(query, key, value, window, sinks=0, lengths=None, scale=None):
+    """One decode step of ``window_attention``: query (B, H, 1, E) over a cache (B, Hkv, S, E) of which
+    sequence b holds its first ``lengths[b]`` rows (int32 or int64 on the GPU; values are clamped to 0 .. S;
+    None: all S), the query's own key the last of them.  Reads the visible rows alone; a sequence of
+    length 0 gives 0.  Head dims up to 256, any strides; forward only."""
+    _check_tensors("attention", query=query, key=key, value=value,
+                   **({} if lengths is None else {"lengths": lengths}))
+    window, sinks, _, scale = _window_numbers(window, sinks, 0, scale)
+    return _native._window_decode(query, key, value, window, sinks, lengths, scale)[0]
+
+
 def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, original_length=None, beta_fast=32.0,
                        beta_slow=1.0, device=None):
     """``(inv_freq, magnitude)`` for ``rotary_embedding`` and ``qk_norm_rotary``: the angle per position
