@@ -953,6 +953,9 @@ dc_status window_args(const dc_window_desc *d, dc::WinArgs *a) {
     return ok();
 }
 
+// The backward's workspace: dsum, then the partials of key tiles that run in pieces.
+size_t window_dsum_ws(const dc::WinArgs &a) { return round_up((size_t)a.B * a.H * a.L * sizeof(float)); }
+
 const char *kWindowNull = "window attention got a null pointer for a non-empty tensor";
 
 dc_status window_decode_args(const dc_window_desc *d, dc::WinDecodeArgs *a) {
@@ -1002,7 +1005,7 @@ dc_status dc_window_fwd(const dc_window_desc *d, const void *q, const void *k, c
 size_t dc_window_bwd_workspace_size(const dc_window_desc *d) {
     dc::WinArgs a;
     if (window_args(d, &a) != DC_OK) return 0;
-    return round_up((size_t)a.B * a.H * a.L * sizeof(float));
+    return window_dsum_ws(a) + round_up(dc::window_bwd_part_bytes(a, d->dtype == DC_BF16));
 }
 
 dc_status dc_window_bwd(const dc_window_desc *d, const void *grad_out, const void *q, const void *k,
@@ -1022,6 +1025,7 @@ dc_status dc_window_bwd(const dc_window_desc *d, const void *grad_out, const voi
     a.dout = grad_out, a.q = q, a.k = k, a.v = v, a.out_in = out, a.lse_in = lse;
     a.dq = dq, a.dk = dk, a.dv = dv;
     a.dsum = static_cast<float *>(workspace);
+    a.kv_part = a.dsum ? a.dsum + window_dsum_ws(a) / sizeof(float) : nullptr;
     a.vec = window_pieces(d, {grad_out, q, k, v, out, dq, dk, dv}, {a.qs, a.ks, a.vs, a.gs});
     return launched(dc::launch_window_bwd(a, d->dtype == DC_BF16, static_cast<hipStream_t>(stream)));
 }

@@ -28,6 +28,11 @@ struct WinArgs {
     float *lse;
     void *dq, *dk, *dv;
     float *dsum;          // (B, H, L): rowsum(dO * O)
+    // dK / dV: the first sink_tiles key tiles (those that hold sinks: every later query sees them) run
+    // as sink_pieces pieces of their queries, the others as tile_pieces, each leaving float32 partials
+    // in kv_part (1: results directly).
+    int sink_tiles, sink_pieces, tile_pieces;
+    float *kv_part;
     bool pack;            // forward: rows of all the heads of a kv head share tiles
     int splits;           // forward: pieces of each tile's keys
     float *part, *part_lse;
@@ -37,6 +42,7 @@ struct WinArgs {
 hipError_t launch_window_fwd(const WinArgs &a, bool bf16, size_t part_bytes, hipStream_t st);
 size_t window_fwd_part_bytes(const WinArgs &a, bool bf16);
 hipError_t launch_window_bwd(const WinArgs &a, bool bf16, hipStream_t st);
+size_t window_bwd_part_bytes(const WinArgs &a, bool bf16);  // of kv_part
 
 struct WinDecodeArgs {
     int B, H, Hkv, S, E, repeat;
@@ -98,13 +104,22 @@ struct Ops<__bf16> {
     DEVI static Frag row(const Tile<R, D> &t, uint32_t base, int row0, int st) { return row_frag<R, D>(t.p, base, row0, st); }
     template <int R, int D>
     DEVI static Frag tr(const Tile<R, D> &t, uint32_t base, int row0, int dt) { return tr_frag<R, D>(t.p, base, row0, dt); }
+    static constexpr int READS = 1, MMAS = 1;  // 16-byte LDS reads of a row fragment, MFMAs of a product
     DEVI static f32x16 mma(Frag a, Frag b, f32x16 c) { return mfma_bf16(a, b, c); }
     DEVI static PFrag split(const f32x16 &x, int at) {
         PFrag p;
         split_bf16(x, at, p.h, p.l);
         return p;
     }
-    DEVI static f32x16 mma_p(Frag a, const PFrag &p, f32x16 c) { return mfma_bf16(a, p.h, mfma_bf16(a, p.l, c)); }
+    // c[i] += a[i] p, the N independent chains product by product.
+    static constexpr int PRODUCTS = 2;
+    template <int N>
+    DEVI static void mma_p(const Frag (&a)[N], const PFrag &p, f32x16 (&c)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) c[i] = mfma_bf16(a[i], p.l, c[i]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) c[i] = mfma_bf16(a[i], p.h, c[i]);
+    }
     // Dims d0 .. d0 + 7 of a row (0 past E, and all 0 without `in`).
     template <bool VEC>
     DEVI static Frag load(const __bf16 *row, int d0, int E, bool in) {
@@ -141,9 +156,17 @@ struct Ops<float> {
     DEVI static Frag row(const Tile<R, D> &t, uint32_t base, int row0, int st) { return row_frag_x3<R, D>(t, base, row0, st); }
     template <int R, int D>
     DEVI static Frag tr(const Tile<R, D> &t, uint32_t base, int row0, int dt) { return tr_frag_x3<R, D>(t, base, row0, dt); }
+    static constexpr int READS = 3, MMAS = 6;
     DEVI static f32x16 mma(const Frag &a, const Frag &b, f32x16 c) { return mfma_x3(a, b, c); }
     DEVI static PFrag split(const f32x16 &x, int at) { return split3(x, at); }
-    DEVI static f32x16 mma_p(const Frag &a, const PFrag &p, f32x16 c) { return mfma_x3(a, p, c); }
+    static constexpr int PRODUCTS = 6;
+    template <int N>
+    DEVI static void mma_p(const Frag (&a)[N], const PFrag &p, f32x16 (&c)[N]) {
+#pragma unroll
+        for (int j = 0; j < 6; ++j)
+#pragma unroll
+            for (int i = 0; i < N; ++i) c[i] = mfma_x3_part(a[i], p, c[i], j);
+    }
     template <bool VEC>
     DEVI static Frag load(const float *row, int d0, int E, bool in) {
         f32x4 x[2];
@@ -236,6 +259,19 @@ struct Stage<float, R, D, THREADS, VEC> {
     }
     DEVI void finish(Tile &t, int tid) { s.store(t, tid); }
 };
+
+// Scheduling hint for a straight run of N steps of M MFMAs, each step consuming R LDS reads: the reads are
+// kept AHEAD steps in front of their use.
+template <int N, int M, int R, int AHEAD>
+DEVI void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, R * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, M * AHEAD, 0);
+}
 
 // Four consecutive dims of a row of a result.
 template <typename T, bool VEC>

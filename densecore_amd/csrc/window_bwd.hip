@@ -18,10 +18,15 @@ namespace {
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kM = 32 * kWaves;
 template <typename T>
 constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // dQ: keys per tile
-template <typename T>
-constexpr int kRows = sizeof(T) == 2 ? 64 : 32;  // dK / dV: queries per step
+// Two waves per SIMD, but for float32 at D = 128 (three parts of two operands and the sums take 350 registers).
 template <typename T, int D>
-constexpr int kWavesPerSimd = D <= 64 && sizeof(T) == 2 ? 2 : 1;
+constexpr int kWavesPerSimd = sizeof(T) == 2 || D <= 64 ? 2 : 1;
+// dK / dV: waves w and w + 4 own the same 32 keys and halve each step's queries (one wave per SIMD: no halves).
+template <typename T, int D>
+constexpr int kHalves = kWavesPerSimd<T, D>;
+// dK / dV: V's operands in LDS (bf16 at D = 128: registers hold K's alone).
+template <typename T, int D>
+constexpr bool kVLds = sizeof(T) == 2 && D == 128;
 
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(kThreads)
@@ -98,19 +103,29 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
                 s = O::mma(O::row(sk[i & 1], rowb, 32 * kt, st), qf[st], s);
                 t = O::mma(O::row(sv[i & 1], rowb, 32 * kt, st), gf[st], t);
             }
+            reads_ahead<2 * KSTEP, O::MMAS, O::READS, sizeof(T) == 2 ? 4 : 2>();
+            __builtin_amdgcn_sched_barrier(0);
+            typename O::Frag kf[2][NDT];  // K^T of the 16-key halves, the first while dS is formed
+            auto load_k = [&](int u) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int key = k0 + acc_row(e, g);
-                float x = fmaf(s[e], a.scale_log2, nlse);
-                const bool hidden = !all && (key >= a.S || !sees(p, key, a.window, a.sinks));
-                s[e] = hidden ? 0.f : exp2_fast(x) * t[e];
+                for (int dt = 0; dt < NDT; ++dt) kf[u][dt] = O::tr(sk[i & 1], trb, 32 * kt + 16 * u, dt);
+            };
+            load_k(0);
+            if (all) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = exp2_fast(fmaf(s[e], a.scale_log2, nlse)) * t[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = k0 + acc_row(e, g);
+                    const float ds = exp2_fast(fmaf(s[e], a.scale_log2, nlse)) * t[e];
+                    s[e] = key < a.S && sees(p, key, a.window, a.sinks) ? ds : 0.f;
+                }
             }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const typename O::PFrag pf = O::split(s, 8 * u);
-#pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) acc[dt] = O::mma_p(O::tr(sk[i & 1], trb, 32 * kt + 16 * u, dt), pf, acc[dt]);
-            }
+            if (sizeof(T) == 2) load_k(1);
+            O::mma_p(kf[0], O::split(s, 0), acc);
+            if (sizeof(T) != 2) load_k(1);
+            O::mma_p(kf[1], O::split(s, 8), acc);
         }
     };
     for (int i = 0; i < band.n; ++i) {
@@ -172,35 +187,74 @@ __host__ __device__ inline void query_range(const WinArgs &a, int n0, int n1, in
     if (l1 < l0) l1 = l0;
 }
 
+// Steps (of QM queries, over the heads that share the kv head) of the key tile at n0.
+__host__ __device__ inline int64_t tile_steps(const WinArgs &a, int n0, int QM) {
+    int l0, l1;
+    query_range(a, n0, n0 + kM < a.S ? n0 + kM : a.S, l0, l1);
+    return (int64_t)((l1 - l0 + QM - 1) / QM) * a.repeat;
+}
+
+// Key tile kt's pieces and the first one's slot in kv_part (a slot: kM keys of dK, then of dV).
+struct Pieces {
+    int n;
+    int64_t slot;
+};
+DEVI Pieces pieces_of(const WinArgs &a, int nkt, int bhk, int kt) {
+    const int64_t head = (int64_t)a.sink_tiles * a.sink_pieces + (int64_t)(nkt - a.sink_tiles) * a.tile_pieces;
+    if (kt < a.sink_tiles) return {a.sink_pieces, bhk * head + (int64_t)kt * a.sink_pieces};
+    return {a.tile_pieces, bhk * head + (int64_t)a.sink_tiles * a.sink_pieces + (int64_t)(kt - a.sink_tiles) * a.tile_pieces};
+}
+
 template <typename T, int D, bool VEC>
-__global__ __launch_bounds__(kThreads)
+__global__ __launch_bounds__((kThreads * kHalves<T, D>))
 __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) void window_dkdv_kernel(WinArgs a) {
     typedef Ops<T> O;
-    constexpr int QM = kRows<T>, NS = QM / 32, KSTEP = D / 16, NDT = D / 32;
-    typedef Stage<T, QM, D, kThreads, VEC> St;
-    __shared__ typename St::Tile sq[2], sg[2];
-    __shared__ float slse[2][QM], sdsum[2][QM];  // -lse log2 e (-inf behind the last row: P = 0) and -dsum
+    constexpr int HALVES = kHalves<T, D>, QM = 32 * HALVES, THREADS = kThreads * HALVES, KSTEP = D / 16, NDT = D / 32;
+    constexpr bool VLDS = kVLds<T, D>;
+    typedef Stage<T, QM, D, THREADS, VEC> St;
+    typedef Stage<T, VLDS ? kM : 32, D, THREADS, VEC> StV;
+    struct Main {
+        typename St::Tile q[2], g[2];
+        float lse[2][QM], dsum[2][QM];  // -lse log2 e (-inf behind the last row: P = 0) and -dsum
+        typename StV::Tile v[VLDS ? 1 : 0];
+    };
+    union Smem {
+        Main m;
+        float red[HALVES - 1][kWaves][NDT][16][64];  // the second half's sums on their way to the first
+    };
+    __shared__ Smem sm;
 
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, g = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave % kWaves, half = wave / kWaves;
     const int nkt = (a.S + kM - 1) / kM;
-    const int w = logical_block();
-    const int n0 = w % nkt * kM, bhk = w / nkt, b = bhk / a.Hkv, hk = bhk % a.Hkv;
-    const int kw0 = n0 + 32 * wave, key = kw0 + lr;
+    const int per = a.sink_tiles * a.sink_pieces + (nkt - a.sink_tiles) * a.tile_pieces;  // blocks of a kv head
+    const int w = logical_block(), bhk = w / per;
+    int kt = w % per, piece;
+    if (kt < a.sink_tiles * a.sink_pieces) {
+        piece = kt % a.sink_pieces, kt = kt / a.sink_pieces;
+    } else {
+        kt -= a.sink_tiles * a.sink_pieces;
+        piece = kt % a.tile_pieces, kt = a.sink_tiles + kt / a.tile_pieces;
+    }
+    const Pieces pcs = pieces_of(a, nkt, bhk, kt);
+    const int n0 = kt * kM, b = bhk / a.Hkv, hk = bhk % a.Hkv;
+    const int kw0 = n0 + 32 * kw, key = kw0 + lr;
     const T *kb = static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[1];
     const T *vb = static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1];
     const T *qb = static_cast<const T *>(a.q) + b * a.qs[0];
     const T *gb = static_cast<const T *>(a.dout) + b * a.gs[0];
     int l0, l1;
     query_range(a, n0, min(n0 + kM, a.S), l0, l1);
-    const int per_head = (l1 - l0 + QM - 1) / QM, steps = per_head * a.repeat;
+    const int per_head = (l1 - l0 + QM - 1) / QM;
+    const int64_t all_steps = (int64_t)per_head * a.repeat;
+    const int i0 = (int)(piece * all_steps / pcs.n), i1 = (int)((piece + 1) * all_steps / pcs.n);
 
     St qst, gst;
     float stat = 0.f;
     auto start = [&](int i) {
         const int h = hk * a.repeat + i / per_head, m0 = l0 + i % per_head * QM, nr = min(QM, a.L - m0);
-        qst.start(sq[i & 1], qb + h * a.qs[1] + m0 * a.qs[2], a.qs[2], nr, a.E, tid);
-        gst.start(sg[i & 1], gb + h * a.gs[1] + m0 * a.gs[2], a.gs[2], nr, a.E, tid);
+        qst.start(sm.m.q[i & 1], qb + h * a.qs[1] + m0 * a.qs[2], a.qs[2], nr, a.E, tid);
+        gst.start(sm.m.g[i & 1], gb + h * a.gs[1] + m0 * a.gs[2], a.gs[2], nr, a.E, tid);
         if (tid < 2 * QM) {
             const int64_t row = ((int64_t)b * a.H + h) * a.L + m0 + tid % QM;
             if (tid < QM) stat = tid < nr ? -a.lse_in[row] * kLog2e : -INFINITY;
@@ -208,21 +262,27 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
         }
     };
     auto finish = [&](int i) {
-        qst.finish(sq[i & 1], tid);
-        gst.finish(sg[i & 1], tid);
-        if (tid < QM) slse[i & 1][tid] = stat;
-        else if (tid < 2 * QM) sdsum[i & 1][tid - QM] = stat;
+        qst.finish(sm.m.q[i & 1], tid);
+        gst.finish(sm.m.g[i & 1], tid);
+        if (tid < QM) sm.m.lse[i & 1][tid] = stat;
+        else if (tid < 2 * QM) sm.m.dsum[i & 1][tid - QM] = stat;
     };
 #pragma unroll
-    for (int i = 0; i < 2; ++i) St::clear(sq[i], a.E, tid), St::clear(sg[i], a.E, tid);
-    if (steps > 0) start(0), finish(0);
+    for (int i = 0; i < 2; ++i) St::clear(sm.m.q[i], a.E, tid), St::clear(sm.m.g[i], a.E, tid);
+    if constexpr (VLDS) {
+        StV vst;
+        StV::clear(sm.m.v[0], a.E, tid);
+        vst.start(sm.m.v[0], vb + (int64_t)n0 * a.vs[2], a.vs[2], min(kM, a.S - n0), a.E, tid);
+        vst.finish(sm.m.v[0], tid);
+    }
+    if (i0 < i1) start(i0), finish(i0);
 
-    typename O::Frag kf[KSTEP], vf[KSTEP];
+    typename O::Frag kf[KSTEP], vf[VLDS ? 1 : KSTEP];
 #pragma unroll
     for (int t = 0; t < KSTEP; ++t) {
         const int kr = min(key, a.S - 1);
         kf[t] = O::template load<VEC>(kb + kr * a.ks[2], 16 * t + 8 * g, a.E, key < a.S);
-        vf[t] = O::template load<VEC>(vb + kr * a.vs[2], 16 * t + 8 * g, a.E, key < a.S);
+        if constexpr (!VLDS) vf[t] = O::template load<VEC>(vb + kr * a.vs[2], 16 * t + 8 * g, a.E, key < a.S);
     }
     f32x16 dk[NDT], dv[NDT];
 #pragma unroll
@@ -230,104 +290,201 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[dt][e] = dv[dt][e] = 0.f;
     const uint32_t rowb = row_lanebase<QM, D>(lane), trb = tr_lanebase<QM, D>(lane);
+    const uint32_t rowv = row_lanebase<VLDS ? kM : 32, D>(lane);
 
     auto step = [&](int i) {
-        const int buf = i & 1, m0 = l0 + i % per_head * QM;
+        const int buf = i & 1, mq = l0 + i % per_head * QM + 32 * half, r0 = 32 * half;
+        const int q0 = a.offset + mq, q1 = a.offset + min(mq + 31, a.L - 1);
+        if (mq >= a.L || kw0 >= a.S || kw0 > q1 || (q0 - (kw0 + 31) >= a.window && kw0 >= a.sinks)) return;
+        const bool all = kw0 + 31 < a.S && kw0 + 31 <= q0 && (q1 - kw0 < a.window || kw0 + 31 < a.sinks);
+        f32x16 s, t;
+        f32x4 nl[4];
 #pragma unroll
-        for (int sub = 0; sub < NS; ++sub) {
-            const int mq = m0 + 32 * sub, q0 = a.offset + mq, q1 = a.offset + min(mq + 31, a.L - 1);
-            if (mq >= a.L || kw0 >= a.S || kw0 > q1 || (q0 - (kw0 + 31) >= a.window && kw0 >= a.sinks)) continue;
-            const bool all = kw0 + 31 < a.S && kw0 + 31 <= q0 && (q1 - kw0 < a.window || kw0 + 31 < a.sinks);
-            f32x16 s, t;
-            f32x4 nl[4];
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int rr = r0 + 8 * r4 + 4 * g;
+            const f32x4 nd = *reinterpret_cast<const f32x4 *>(&sm.m.dsum[buf][rr]);
+            nl[r4] = *reinterpret_cast<const f32x4 *>(&sm.m.lse[buf][rr]);
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const int rr = 32 * sub + 8 * r4 + 4 * g;
-                const f32x4 nd = *reinterpret_cast<const f32x4 *>(&sdsum[buf][rr]);
-                nl[r4] = *reinterpret_cast<const f32x4 *>(&slse[buf][rr]);
+            for (int j = 0; j < 4; ++j) s[4 * r4 + j] = 0.f, t[4 * r4 + j] = nd[j];
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[4 * r4 + j] = 0.f, t[4 * r4 + j] = nd[j];
-            }
+        for (int st = 0; st < KSTEP; ++st) {
+            s = O::mma(O::row(sm.m.q[buf], rowb, r0, st), kf[st], s);
+            if constexpr (VLDS) t = O::mma(O::row(sm.m.g[buf], rowb, r0, st), O::row(sm.m.v[0], rowv, 32 * kw, st), t);
+            else t = O::mma(O::row(sm.m.g[buf], rowb, r0, st), vf[st], t);
+        }
+        reads_ahead<KSTEP, 2 * O::MMAS, (VLDS ? 3 : 2) * O::READS, sizeof(T) == 2 ? 2 : 1>();
+        __builtin_amdgcn_sched_barrier(0);
+        // dV^T += dO^T P and dK^T += Q^T dS, 16 queries at a time; bf16's transposed operands are read a
+        // product ahead, the first while P and dS are formed.
+        typename O::Frag f[2][NDT];
+        auto load = [&](int n) {
 #pragma unroll
-            for (int st = 0; st < KSTEP; ++st) {
-                s = O::mma(O::row(sq[buf], rowb, 32 * sub, st), kf[st], s);
-                t = O::mma(O::row(sg[buf], rowb, 32 * sub, st), vf[st], t);
-            }
+            for (int dt = 0; dt < NDT; ++dt)
+                f[n & 1][dt] = O::tr((n & 1) ? sm.m.q[buf] : sm.m.g[buf], trb, r0 + 16 * (n >> 1), dt);
+        };
+        load(0);
+        if (all) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const int qp = q0 + acc_row(e, g);
-                const bool hidden = !all && (key >= a.S || !sees(qp, key, a.window, a.sinks));
-                const float pr = hidden ? 0.f : exp2_fast(fmaf(s[e], a.scale_log2, nl[e >> 2][e & 3]));
-                s[e] = pr;
-                t[e] = hidden ? 0.f : pr * t[e];
+                s[e] = exp2_fast(fmaf(s[e], a.scale_log2, nl[e >> 2][e & 3]));
+                t[e] *= s[e];
             }
+        } else {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const typename O::PFrag pf = O::split(s, 8 * u), df = O::split(t, 8 * u);
-#pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) dv[dt] = O::mma_p(O::tr(sg[buf], trb, 32 * sub + 16 * u, dt), pf, dv[dt]);
-#pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) dk[dt] = O::mma_p(O::tr(sq[buf], trb, 32 * sub + 16 * u, dt), df, dk[dt]);
+            for (int e = 0; e < 16; ++e) {
+                const bool seen = key < a.S && sees(q0 + acc_row(e, g), key, a.window, a.sinks);
+                const float pr = exp2_fast(fmaf(s[e], a.scale_log2, nl[e >> 2][e & 3]));
+                s[e] = seen ? pr : 0.f;
+                t[e] = seen ? pr * t[e] : 0.f;
             }
         }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            if (sizeof(T) == 2 && n + 1 < 4) load(n + 1);
+            if (n & 1) O::mma_p(f[n & 1], O::split(t, 8 * (n >> 1)), dk);
+            else O::mma_p(f[n & 1], O::split(s, 8 * (n >> 1)), dv);
+            if (sizeof(T) != 2 && n + 1 < 4) load(n + 1);
+        }
     };
-    for (int i = 0; i < steps; ++i) {
+    for (int i = i0; i < i1; ++i) {
         __syncthreads();
-        if (i + 1 < steps) start(i + 1);
+        if (i + 1 < i1) start(i + 1);
         step(i);
-        if (i + 1 < steps) finish(i + 1);
+        if (i + 1 < i1) finish(i + 1);
     }
 
+    if constexpr (HALVES == 2) {  // the second half's sums join the first's, dK then dV through the same room
+        auto join = [&](f32x16 (&x)[NDT]) {
+            __syncthreads();
+            if (half == 1) {
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sm.red[0][kw][dt][e][lane] = x[dt][e];
+            }
+            __syncthreads();
+            if (half == 0) {
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[dt][e] += sm.red[0][kw][dt][e][lane];
+            }
+        };
+        join(dk), join(dv);
+        if (half == 1) return;
+    }
     float test = 0.f;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) test += not_finite(dk[dt]) + not_finite(dv[dt]);
     const uint64_t wrong = __ballot(key < a.S && test != 0.f);
     uint32_t again = (uint32_t)wrong | (uint32_t)(wrong >> 32);
-    T *dko = static_cast<T *>(a.dk) + (int64_t)bhk * a.S * a.E, *dvo = static_cast<T *>(a.dv) + (int64_t)bhk * a.S * a.E;
+    // Rows of this block: results, or its piece's float32 slot.
+    T *dko = static_cast<T *>(a.dk) + ((int64_t)bhk * a.S + n0) * a.E, *dvo = static_cast<T *>(a.dv) + ((int64_t)bhk * a.S + n0) * a.E;
+    float *pk = a.kv_part + (pcs.slot + piece) * 2 * kM * a.E, *pv = pk + (int64_t)kM * a.E;
+    const int at = 32 * kw + lr;
     if (key < a.S && !((again >> lr) & 1)) {
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const int d = dt * 32 + acc_row(e, g);
-                store4<T, VEC>(dko + (int64_t)key * a.E, d, a.E, dk[dt][e] * a.scale, dk[dt][e + 1] * a.scale,
-                               dk[dt][e + 2] * a.scale, dk[dt][e + 3] * a.scale);
-                store4<T, VEC>(dvo + (int64_t)key * a.E, d, a.E, dv[dt][e], dv[dt][e + 1], dv[dt][e + 2], dv[dt][e + 3]);
+                float x[4], y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = dk[dt][e + j] * a.scale, y[j] = dv[dt][e + j];
+                if (pcs.n > 1) {
+                    store4<float, VEC>(pk + at * a.E, d, a.E, x[0], x[1], x[2], x[3]);
+                    store4<float, VEC>(pv + at * a.E, d, a.E, y[0], y[1], y[2], y[3]);
+                } else {
+                    store4<T, VEC>(dko + (int64_t)at * a.E, d, a.E, x[0], x[1], x[2], x[3]);
+                    store4<T, VEC>(dvo + (int64_t)at * a.E, d, a.E, y[0], y[1], y[2], y[3]);
+                }
             }
     }
-    // Keys again: lanes are queries for P and dS and dims for the sums.
+    // Keys again, over this block's steps: lanes are queries for P and dS and dims for the sums.
     for (; again; again &= again - 1) {
-        const int rk = kw0 + __builtin_ctz(again);
+        const int ra = 32 * kw + __builtin_ctz(again), rk = n0 + ra;
         const T *k1 = kb + rk * a.ks[2], *v1 = vb + rk * a.vs[2];
         float xk[2] = {0.f, 0.f}, xv[2] = {0.f, 0.f};
-        for (int i = 0; i < a.repeat; ++i) {
-            const int h = hk * a.repeat + i;
-            for (int m = l0; m < l1; m += 64) {
-                const int l = m + lane;
-                const bool ok = l < l1 && sees(a.offset + l, rk, a.window, a.sinks);
-                float pr = 0.f, ds = 0.f;
-                if (ok) {
-                    const int64_t row = ((int64_t)b * a.H + h) * a.L + l;
-                    pr = exp2_fast((plain_dot<T>(qb + h * a.qs[1] + l * a.qs[2], k1, a.E) * a.scale - a.lse_in[row]) * kLog2e);
-                    ds = pr * (plain_dot<T>(gb + h * a.gs[1] + l * a.gs[2], v1, a.E) - a.dsum[row]);
-                }
-                for (uint64_t left = __ballot(ok); left; left &= left - 1) {
-                    const int j = __builtin_ctzll(left);
-                    const float pj = __shfl(pr, j, 64), dj = __shfl(ds, j, 64);
-                    const T *q1 = qb + h * a.qs[1] + (m + j) * a.qs[2], *g1 = gb + h * a.gs[1] + (m + j) * a.gs[2];
+        for (int i = i0; i < i1; ++i) {
+            const int h = hk * a.repeat + i / per_head, m = l0 + i % per_head * QM, l = m + lane;
+            const bool ok = lane < QM && l < a.L && sees(a.offset + l, rk, a.window, a.sinks);
+            float pr = 0.f, ds = 0.f;
+            if (ok) {
+                const int64_t row = ((int64_t)b * a.H + h) * a.L + l;
+                pr = exp2_fast((plain_dot<T>(qb + h * a.qs[1] + l * a.qs[2], k1, a.E) * a.scale - a.lse_in[row]) * kLog2e);
+                ds = pr * (plain_dot<T>(gb + h * a.gs[1] + l * a.gs[2], v1, a.E) - a.dsum[row]);
+            }
+            for (uint64_t left = __ballot(ok); left; left &= left - 1) {
+                const int j = __builtin_ctzll(left);
+                const float pj = __shfl(pr, j, 64), dj = __shfl(ds, j, 64);
+                const T *q1 = qb + h * a.qs[1] + (m + j) * a.qs[2], *g1 = gb + h * a.gs[1] + (m + j) * a.gs[2];
 #pragma unroll
-                    for (int d = lane, n = 0; n < 2; ++n, d += 64)
-                        if (d < a.E) xk[n] = fmaf(dj, to_f32<T>(q1[d]), xk[n]), xv[n] = fmaf(pj, to_f32<T>(g1[d]), xv[n]);
-                }
+                for (int d = lane, n = 0; n < 2; ++n, d += 64)
+                    if (d < a.E) xk[n] = fmaf(dj, to_f32<T>(q1[d]), xk[n]), xv[n] = fmaf(pj, to_f32<T>(g1[d]), xv[n]);
             }
         }
 #pragma unroll
         for (int d = lane, n = 0; n < 2; ++n, d += 64)
             if (d < a.E) {
-                dko[(int64_t)rk * a.E + d] = from_f32<T>(xk[n] * a.scale);
-                dvo[(int64_t)rk * a.E + d] = from_f32<T>(xv[n]);
+                if (pcs.n > 1) {
+                    pk[ra * a.E + d] = xk[n] * a.scale, pv[ra * a.E + d] = xv[n];
+                } else {
+                    dko[(int64_t)ra * a.E + d] = from_f32<T>(xk[n] * a.scale);
+                    dvo[(int64_t)ra * a.E + d] = from_f32<T>(xv[n]);
+                }
             }
     }
+}
+
+// The pieces of each key row summed in order, one thread per 4 dims of a row of dK or dV: the first `rows`
+// keys of every kv head.
+template <typename T>
+__global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, int rows) {
+    const int groups = (a.E + 3) / 4, nkt = (a.S + kM - 1) / kM;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)a.B * a.Hkv * rows * groups * 2;
+    if (id >= n) return;
+    const int d = (int)(id % groups) * 4, which = (int)(id / groups % 2);
+    const int64_t r = id / groups / 2;
+    const int key = (int)(r % rows), bhk = (int)(r / rows);
+    const Pieces pcs = pieces_of(a, nkt, bhk, key / kM);
+    const float *src = a.kv_part + (pcs.slot * 2 + which) * kM * a.E + (int64_t)(key % kM) * a.E + d;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < pcs.n; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < a.E) x[e] += src[(int64_t)i * 2 * kM * a.E + e];
+    T *dst = static_cast<T *>(which ? a.dv : a.dk) + ((int64_t)bhk * a.S + key) * a.E;
+    store4<T, false>(dst, d, a.E, x[0], x[1], x[2], x[3]);
+}
+
+// How the dK / dV grid is cut.  A tile of sinks has the queries of the whole sequence where the others have a
+// window's: pieces of about as many steps as those.  And where the blocks do not fill the CUs, pieces
+// of at least 4 steps that do.
+void plan_pieces(WinArgs &a, bool bf16) {
+    const int QM = 32 * (bf16 || a.E <= 64 ? 2 : 1), nkt = (a.S + kM - 1) / kM;
+    a.sink_tiles = (int)std::min<int64_t>(nkt, ((int64_t)a.sinks + kM - 1) / kM);
+    a.sink_pieces = a.tile_pieces = 1;
+    if (nkt == 0 || a.L == 0 || a.B * a.Hkv == 0) return;
+    int64_t most = 0;  // steps of the longest tile without sinks
+    for (int kt = a.sink_tiles; kt < nkt; ++kt) most = std::max(most, tile_steps(a, kt * kM, QM));
+    const int64_t heads = (int64_t)a.B * a.Hkv, cus = std::max(device_cus(), 1), rest = nkt - a.sink_tiles;
+    if (rest > 0 && most > 0)
+        a.tile_pieces = (int)std::max<int64_t>(1, std::min<int64_t>(most / 4, cus / (heads * rest)));
+    const int64_t sink = a.sink_tiles > 0 ? tile_steps(a, 0, QM) : 0;
+    const int64_t piece = std::max<int64_t>(4, rest > 0 && most > 0 ? (most + a.tile_pieces - 1) / a.tile_pieces : sink);
+    if (rest == 0 && sink > 0) {
+        a.sink_pieces = (int)std::max<int64_t>(1, std::min<int64_t>(sink / 4, cus / (heads * a.sink_tiles)));
+    } else if (sink > 0) {  // (no more than 4 blocks per CU: the partials stay below 140 MB)
+        const int64_t room = 4 * cus / (heads * a.sink_tiles);
+        a.sink_pieces = (int)std::max<int64_t>(1, std::min<int64_t>(room, (sink + piece - 1) / piece));
+    }
+}
+
+int64_t blocks_per_head(const WinArgs &a) {
+    const int nkt = (a.S + kM - 1) / kM;
+    return (int64_t)a.sink_tiles * a.sink_pieces + (int64_t)(nkt - a.sink_tiles) * a.tile_pieces;
 }
 
 template <typename T, int D, bool VEC>
@@ -335,10 +492,13 @@ hipError_t launch_v(const WinArgs &a, hipStream_t st) {
     if (a.L > 0)
         return_if(launch(window_dq_kernel<T, D, VEC>, dim3((unsigned)((int64_t)(a.L + kM - 1) / kM * a.B * a.H)), dim3(kThreads),
                          st, a));
-    if (a.S > 0)
-        return_if(launch(window_dkdv_kernel<T, D, VEC>, dim3((unsigned)((int64_t)(a.S + kM - 1) / kM * a.B * a.Hkv)),
-                         dim3(kThreads), st, a));
-    return hipSuccess;
+    if (a.S == 0) return hipSuccess;
+    return_if(launch(window_dkdv_kernel<T, D, VEC>, dim3((unsigned)(blocks_per_head(a) * a.B * a.Hkv)),
+                     dim3(kThreads * kHalves<T, D>), st, a));
+    const int rows = a.tile_pieces > 1 ? a.S : a.sink_pieces > 1 ? std::min(a.S, a.sink_tiles * kM) : 0;
+    if (rows == 0) return hipSuccess;
+    const int64_t n = (int64_t)a.B * a.Hkv * rows * ((a.E + 3) / 4) * 2;
+    return launch(window_join_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), st, a, rows);
 }
 template <typename T, int D>
 hipError_t launch_d(const WinArgs &a, hipStream_t st) {
@@ -353,7 +513,16 @@ hipError_t launch_t(const WinArgs &a, hipStream_t st) {
 
 }  // namespace
 
-hipError_t launch_window_bwd(const WinArgs &a, bool bf16, hipStream_t st) {
+size_t window_bwd_part_bytes(const WinArgs &args, bool bf16) {
+    WinArgs a = args;
+    plan_pieces(a, bf16);
+    if (a.sink_pieces == 1 && a.tile_pieces == 1) return 0;
+    return (size_t)(blocks_per_head(a) * a.B * a.Hkv) * 2 * kM * a.E * sizeof(float);
+}
+
+hipError_t launch_window_bwd(const WinArgs &args, bool bf16, hipStream_t st) {
+    WinArgs a = args;
+    plan_pieces(a, bf16);
     return bf16 ? launch_t<__bf16>(a, st) : launch_t<float>(a, st);
 }
 

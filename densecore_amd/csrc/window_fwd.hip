@@ -150,9 +150,20 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
         for (int kt = 0; kt < NT; ++kt) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[kt][e] = 0.f;
-            if (!live[kt]) continue;
+        }
+        if (live[0] && live[NT - 1]) {
 #pragma unroll
-            for (int st = 0; st < KSTEP; ++st) s[kt] = O::mma(O::row(sk[buf], rowb, 32 * kt, st), qf[st], s[kt]);
+            for (int st = 0; st < KSTEP; ++st)
+#pragma unroll
+                for (int kt = 0; kt < NT; ++kt) s[kt] = O::mma(O::row(sk[buf], rowb, 32 * kt, st), qf[st], s[kt]);
+            reads_ahead<KSTEP * NT, O::MMAS, O::READS, sizeof(T) == 2 ? 4 : 2>();
+        } else {
+#pragma unroll
+            for (int kt = 0; kt < NT; ++kt) {
+                if (!live[kt]) continue;
+#pragma unroll
+                for (int st = 0; st < KSTEP; ++st) s[kt] = O::mma(O::row(sk[buf], rowb, 32 * kt, st), qf[st], s[kt]);
+            }
         }
         const bool all = n0 + BN <= a.S && n0 + BN - 1 <= wp0 && (wp1 - n0 < a.window || n0 + BN <= a.sinks);
         if (!all) {
@@ -192,9 +203,10 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
             if (!live[kt]) continue;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const typename O::PFrag pf = O::split(s[kt], 8 * u);
+                typename O::Frag vf[NDT];
 #pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) acc[dt] = O::mma_p(O::tr(sv[buf], trb, 32 * kt + 16 * u, dt), pf, acc[dt]);
+                for (int dt = 0; dt < NDT; ++dt) vf[dt] = O::tr(sv[buf], trb, 32 * kt + 16 * u, dt);
+                O::mma_p(vf, O::split(s[kt], 8 * u), acc);
             }
         }
     };
