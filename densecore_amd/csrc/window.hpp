@@ -273,6 +273,10 @@ DEVI void reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x008, M * AHEAD, 0);
 }
 
+// The products that form x come before what follows in program order: the compiler places them by their
+// first use, behind scheduling hints and barriers, and then all of their operands' reads before them.
+DEVI void pin(f32x16 &x) { asm volatile("" : "+v"(x)); }
+
 // Four consecutive dims of a row of a result.
 template <typename T, bool VEC>
 DEVI void store4(T *row, int d, int E, float x0, float x1, float x2, float x3) {

@@ -24,9 +24,9 @@ constexpr int kWavesPerSimd = sizeof(T) == 2 || D <= 64 ? 2 : 1;
 // dK / dV: waves w and w + 4 own the same 32 keys and halve each step's queries (one wave per SIMD: no halves).
 template <typename T, int D>
 constexpr int kHalves = kWavesPerSimd<T, D>;
-// dK / dV: V's operands in LDS (bf16 at D = 128: registers hold K's alone).
+// dK / dV: K's and V's operands in LDS and not in registers (bf16 at D = 128, where the sums take half of them).
 template <typename T, int D>
-constexpr bool kVLds = sizeof(T) == 2 && D == 128;
+constexpr bool kKvLds = sizeof(T) == 2 && D == 128;
 
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(kThreads)
@@ -104,6 +104,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
                 t = O::mma(O::row(sv[i & 1], rowb, 32 * kt, st), gf[st], t);
             }
             reads_ahead<2 * KSTEP, O::MMAS, O::READS, sizeof(T) == 2 ? 4 : 2>();
+            pin(s), pin(t);
             __builtin_amdgcn_sched_barrier(0);
             typename O::Frag kf[2][NDT];  // K^T of the 16-key halves, the first while dS is formed
             auto load_k = [&](int u) {
@@ -210,13 +211,13 @@ __global__ __launch_bounds__((kThreads * kHalves<T, D>))
 __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) void window_dkdv_kernel(WinArgs a) {
     typedef Ops<T> O;
     constexpr int HALVES = kHalves<T, D>, QM = 32 * HALVES, THREADS = kThreads * HALVES, KSTEP = D / 16, NDT = D / 32;
-    constexpr bool VLDS = kVLds<T, D>;
+    constexpr bool KVLDS = kKvLds<T, D>;
     typedef Stage<T, QM, D, THREADS, VEC> St;
-    typedef Stage<T, VLDS ? kM : 32, D, THREADS, VEC> StV;
+    typedef Stage<T, KVLDS ? kM : 32, D, THREADS, VEC> StV;
     struct Main {
         typename St::Tile q[2], g[2];
         float lse[2][QM], dsum[2][QM];  // -lse log2 e (-inf behind the last row: P = 0) and -dsum
-        typename StV::Tile v[VLDS ? 1 : 0];
+        typename StV::Tile k[KVLDS ? 1 : 0], v[KVLDS ? 1 : 0];
     };
     union Smem {
         Main m;
@@ -251,38 +252,46 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
 
     St qst, gst;
     float stat = 0.f;
-    auto start = [&](int i) {
-        const int h = hk * a.repeat + i / per_head, m0 = l0 + i % per_head * QM, nr = min(QM, a.L - m0);
+    // Step i's head and first query; at(i + 1) is at(i) moved on.
+    struct At {
+        int h, m;
+    };
+    auto first = [&](int i) { return At{hk * a.repeat + i / per_head, l0 + i % per_head * QM}; };
+    auto next = [&](At x) { return x.m + QM < l1 ? At{x.h, x.m + QM} : At{x.h + 1, l0}; };
+    auto start = [&](int i, At x) {
+        const int h = x.h, m0 = x.m, nr = min(QM, a.L - m0);
         qst.start(sm.m.q[i & 1], qb + h * a.qs[1] + m0 * a.qs[2], a.qs[2], nr, a.E, tid);
         gst.start(sm.m.g[i & 1], gb + h * a.gs[1] + m0 * a.gs[2], a.gs[2], nr, a.E, tid);
-        if (tid < 2 * QM) {
-            const int64_t row = ((int64_t)b * a.H + h) * a.L + m0 + tid % QM;
-            if (tid < QM) stat = tid < nr ? -a.lse_in[row] * kLog2e : -INFINITY;
-            else stat = tid - QM < nr ? -a.dsum[row] : 0.f;
-        }
+        // (As it lies: arithmetic on it here would wait for every transfer issued so far.)
+        if (tid < 2 * QM) stat = (tid < QM ? a.lse_in : a.dsum)[((int64_t)b * a.H + h) * a.L + m0 + min(tid % QM, nr - 1)];
     };
-    auto finish = [&](int i) {
+    auto finish = [&](int i, At x) {
         qst.finish(sm.m.q[i & 1], tid);
         gst.finish(sm.m.g[i & 1], tid);
-        if (tid < QM) sm.m.lse[i & 1][tid] = stat;
-        else if (tid < 2 * QM) sm.m.dsum[i & 1][tid - QM] = stat;
+        if (tid < QM) sm.m.lse[i & 1][tid] = x.m + tid < a.L ? -stat * kLog2e : -INFINITY;
+        else if (tid < 2 * QM) sm.m.dsum[i & 1][tid - QM] = x.m + tid - QM < a.L ? -stat : 0.f;
     };
 #pragma unroll
     for (int i = 0; i < 2; ++i) St::clear(sm.m.q[i], a.E, tid), St::clear(sm.m.g[i], a.E, tid);
-    if constexpr (VLDS) {
-        StV vst;
-        StV::clear(sm.m.v[0], a.E, tid);
+    if constexpr (KVLDS) {
+        StV kst, vst;
+        StV::clear(sm.m.k[0], a.E, tid), StV::clear(sm.m.v[0], a.E, tid);
+        kst.start(sm.m.k[0], kb + (int64_t)n0 * a.ks[2], a.ks[2], min(kM, a.S - n0), a.E, tid);
+        kst.finish(sm.m.k[0], tid);
         vst.start(sm.m.v[0], vb + (int64_t)n0 * a.vs[2], a.vs[2], min(kM, a.S - n0), a.E, tid);
         vst.finish(sm.m.v[0], tid);
     }
-    if (i0 < i1) start(i0), finish(i0);
+    At now = {0, 0};
+    if (i0 < i1) now = first(i0), start(i0, now), finish(i0, now);
 
-    typename O::Frag kf[KSTEP], vf[VLDS ? 1 : KSTEP];
+    typename O::Frag kf[KVLDS ? 1 : KSTEP], vf[KVLDS ? 1 : KSTEP];
+    if constexpr (!KVLDS) {
 #pragma unroll
-    for (int t = 0; t < KSTEP; ++t) {
-        const int kr = min(key, a.S - 1);
-        kf[t] = O::template load<VEC>(kb + kr * a.ks[2], 16 * t + 8 * g, a.E, key < a.S);
-        if constexpr (!VLDS) vf[t] = O::template load<VEC>(vb + kr * a.vs[2], 16 * t + 8 * g, a.E, key < a.S);
+        for (int t = 0; t < KSTEP; ++t) {
+            const int kr = min(key, a.S - 1);
+            kf[t] = O::template load<VEC>(kb + kr * a.ks[2], 16 * t + 8 * g, a.E, key < a.S);
+            vf[t] = O::template load<VEC>(vb + kr * a.vs[2], 16 * t + 8 * g, a.E, key < a.S);
+        }
     }
     f32x16 dk[NDT], dv[NDT];
 #pragma unroll
@@ -290,31 +299,33 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[dt][e] = dv[dt][e] = 0.f;
     const uint32_t rowb = row_lanebase<QM, D>(lane), trb = tr_lanebase<QM, D>(lane);
-    const uint32_t rowv = row_lanebase<VLDS ? kM : 32, D>(lane);
+    const uint32_t rowk = row_lanebase<KVLDS ? kM : 32, D>(lane);
 
-    auto step = [&](int i) {
-        const int buf = i & 1, mq = l0 + i % per_head * QM + 32 * half, r0 = 32 * half;
+    auto step = [&](int i, At x) {
+        const int buf = i & 1, mq = x.m + 32 * half, r0 = 32 * half;
         const int q0 = a.offset + mq, q1 = a.offset + min(mq + 31, a.L - 1);
         if (mq >= a.L || kw0 >= a.S || kw0 > q1 || (q0 - (kw0 + 31) >= a.window && kw0 >= a.sinks)) return;
         const bool all = kw0 + 31 < a.S && kw0 + 31 <= q0 && (q1 - kw0 < a.window || kw0 + 31 < a.sinks);
         f32x16 s, t;
-        f32x4 nl[4];
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-            const int rr = r0 + 8 * r4 + 4 * g;
-            const f32x4 nd = *reinterpret_cast<const f32x4 *>(&sm.m.dsum[buf][rr]);
-            nl[r4] = *reinterpret_cast<const f32x4 *>(&sm.m.lse[buf][rr]);
+            const f32x4 nd = *reinterpret_cast<const f32x4 *>(&sm.m.dsum[buf][r0 + 8 * r4 + 4 * g]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[4 * r4 + j] = 0.f, t[4 * r4 + j] = nd[j];
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int st = 0; st < KSTEP; ++st) {
-            s = O::mma(O::row(sm.m.q[buf], rowb, r0, st), kf[st], s);
-            if constexpr (VLDS) t = O::mma(O::row(sm.m.g[buf], rowb, r0, st), O::row(sm.m.v[0], rowv, 32 * kw, st), t);
-            else t = O::mma(O::row(sm.m.g[buf], rowb, r0, st), vf[st], t);
+            if constexpr (KVLDS) {
+                s = O::mma(O::row(sm.m.q[buf], rowb, r0, st), O::row(sm.m.k[0], rowk, 32 * kw, st), s);
+                t = O::mma(O::row(sm.m.g[buf], rowb, r0, st), O::row(sm.m.v[0], rowk, 32 * kw, st), t);
+            } else {
+                s = O::mma(O::row(sm.m.q[buf], rowb, r0, st), kf[st], s);
+                t = O::mma(O::row(sm.m.g[buf], rowb, r0, st), vf[st], t);
+            }
         }
-        reads_ahead<KSTEP, 2 * O::MMAS, (VLDS ? 3 : 2) * O::READS, sizeof(T) == 2 ? 2 : 1>();
+        reads_ahead<KSTEP, 2 * O::MMAS, (KVLDS ? 4 : 2) * O::READS, sizeof(T) == 2 ? 2 : 1>();
+        pin(s), pin(t);
         __builtin_amdgcn_sched_barrier(0);
         // dV^T += dO^T P and dK^T += Q^T dS, 16 queries at a time; bf16's transposed operands are read a
         // product ahead, the first while P and dS are formed.
@@ -324,6 +335,9 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
             for (int dt = 0; dt < NDT; ++dt)
                 f[n & 1][dt] = O::tr((n & 1) ? sm.m.q[buf] : sm.m.g[buf], trb, r0 + 16 * (n >> 1), dt);
         };
+        f32x4 nl[4];
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) nl[r4] = *reinterpret_cast<const f32x4 *>(&sm.m.lse[buf][r0 + 8 * r4 + 4 * g]);
         load(0);
         if (all) {
 #pragma unroll
@@ -346,13 +360,18 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
             if (n & 1) O::mma_p(f[n & 1], O::split(t, 8 * (n >> 1)), dk);
             else O::mma_p(f[n & 1], O::split(s, 8 * (n >> 1)), dv);
             if (sizeof(T) != 2 && n + 1 < 4) load(n + 1);
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) pin((n & 1) ? dk[dt] : dv[dt]);
+            __builtin_amdgcn_sched_barrier(0);  // or all four reads are issued at once, into spilled registers
         }
     };
     for (int i = i0; i < i1; ++i) {
         __syncthreads();
-        if (i + 1 < i1) start(i + 1);
-        step(i);
-        if (i + 1 < i1) finish(i + 1);
+        const At then = next(now);
+        if (i + 1 < i1) start(i + 1, then);
+        step(i, now);
+        if (i + 1 < i1) finish(i + 1, then);
+        now = then;
     }
 
     if constexpr (HALVES == 2) {  // the second half's sums join the first's, dK then dV through the same room

@@ -157,6 +157,9 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
 #pragma unroll
                 for (int kt = 0; kt < NT; ++kt) s[kt] = O::mma(O::row(sk[buf], rowb, 32 * kt, st), qf[st], s[kt]);
             reads_ahead<KSTEP * NT, O::MMAS, O::READS, sizeof(T) == 2 ? 4 : 2>();
+#pragma unroll
+            for (int kt = 0; kt < NT; ++kt) pin(s[kt]);
+            __builtin_amdgcn_sched_barrier(0);
         } else {
 #pragma unroll
             for (int kt = 0; kt < NT; ++kt) {
