@@ -138,8 +138,8 @@ def lib():
         for name in ("dc_window_fwd", "dc_window_bwd", "dc_window_decode"):
             getattr(L, name + "_workspace_size").argtypes = [WD]
             getattr(L, name + "_workspace_size").restype = SZ
-        L.dc_window_fwd.argtypes = [WD, P, P, P, P, P, P, SZ, P]
-        L.dc_window_bwd.argtypes = [WD] + [P] * 10 + [SZ, P]
+        L.dc_window_fwd.argtypes = [WD, P, P, P, P, P, P, P, SZ, P]
+        L.dc_window_bwd.argtypes = [WD] + [P] * 11 + [SZ, P]
         L.dc_window_decode.argtypes = [WD, P, P, P, P, ctypes.c_int32, P, P, P, SZ, P]
         for name in ("dc_window_fwd", "dc_window_bwd", "dc_window_decode", "dc_rotary_fwd", "dc_rotary_bwd",
                      "dc_sdpa_fwd", "dc_sdpa_bwd", "dc_sdpa_decode", "dc_softmax_fwd",

@@ -437,23 +437,25 @@ def _window_desc(q, k, v, window, sinks, offset, scale, grad_out=None):
                            *(S3(*t.stride()[:3]) if t is not None else S3() for t in (q, k, v, grad_out)))
 
 
-def _window_attention(q, k, v, window, sinks=0, offset=0, scale=None):
-    """``dc_window_fwd``: (out, lse)."""
+def _window_attention(q, k, v, window, sinks=0, offset=0, scale=None, with_rest=False):
+    """``dc_window_fwd``: (out, lse), with ``with_rest`` (out, lse, rest): for the backward, what rounding
+    a bf16 out left (None for float32)."""
     q, k, v = _unit_rows(q), _unit_rows(k), _unit_rows(v)
     d = _window_desc(q, k, v, window, sinks, offset, scale)
     dev, L_ = q.device, _lib.lib()
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
+    rest = torch.empty_like(out) if with_rest and q.dtype == torch.bfloat16 else None
     with _on(dev):
         nbytes = L_.dc_window_fwd_workspace_size(d)
         ws = _workspace(nbytes, dev) if nbytes else None
-        _lib.check(L_.dc_window_fwd(d, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(ws),
+        _lib.check(L_.dc_window_fwd(d, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(lse), _ptr(ws),
                                     0 if ws is None else ws.numel(), _stream(dev)))
-    return out, lse
+    return (out, lse, rest) if with_rest else (out, lse)
 
 
-def _window_attention_backward(grad_out, q, k, v, out, lse, window, sinks=0, offset=0, scale=None):
-    """``dc_window_bwd``: (dq, dk, dv)."""
+def _window_attention_backward(grad_out, q, k, v, out, lse, rest, window, sinks=0, offset=0, scale=None):
+    """``dc_window_bwd``: (dq, dk, dv); ``rest`` as the forward gave it, or None."""
     grad_out, q, k, v = (_unit_rows(t) for t in (grad_out, q, k, v))
     d = _window_desc(q, k, v, window, sinks, offset, scale, grad_out)
     dev, L_ = q.device, _lib.lib()
@@ -461,12 +463,14 @@ def _window_attention_backward(grad_out, q, k, v, out, lse, window, sinks=0, off
         raise ValueError("window attention backward shapes do not match")
     if out.device != dev or lse.device != dev:
         raise ValueError("window attention tensors must share one device and dtype")
-    out, lse = out.contiguous(), lse.contiguous()
+    if rest is not None and (rest.shape != q.shape or rest.dtype != q.dtype or rest.device != dev):
+        raise ValueError("window attention backward shapes do not match")
+    out, lse, rest = out.contiguous(), lse.contiguous(), None if rest is None else rest.contiguous()
     dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v))
     with _on(dev):
         ws = _workspace(L_.dc_window_bwd_workspace_size(d), dev)
-        _lib.check(L_.dc_window_bwd(d, _ptr(grad_out), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq),
-                                    _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream(dev)))
+        _lib.check(L_.dc_window_bwd(d, _ptr(grad_out), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(lse),
+                                    _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream(dev)))
     return dq, dk, dv
 
 

@@ -988,7 +988,7 @@ size_t dc_window_fwd_workspace_size(const dc_window_desc *d) {
 }
 
 dc_status dc_window_fwd(const dc_window_desc *d, const void *q, const void *k, const void *v, void *out,
-                        float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+                        void *rest, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
     dc::WinArgs a;
     dc_status st = window_args(d, &a);
     if (st != DC_OK) return st;
@@ -996,8 +996,8 @@ dc_status dc_window_fwd(const dc_window_desc *d, const void *q, const void *k, c
     if (nq == 0) return ok();
     if (!present(q, nq * a.E) || !present(k, nkv) || !present(v, nkv) || !present(out, nq * a.E) || lse == nullptr)
         return fail(DC_INVALID_ARGUMENT, kWindowNull);
-    a.q = q, a.k = k, a.v = v, a.out = out, a.lse = lse;
-    a.vec = window_pieces(d, {q, k, v, out}, {a.qs, a.ks, a.vs});
+    a.q = q, a.k = k, a.v = v, a.out = out, a.rest = rest, a.lse = lse;
+    a.vec = window_pieces(d, {q, k, v, out, rest}, {a.qs, a.ks, a.vs});
     a.part = static_cast<float *>(workspace);
     return launched(dc::launch_window_fwd(a, d->dtype == DC_BF16, workspace_bytes, static_cast<hipStream_t>(stream)));
 }
@@ -1009,7 +1009,7 @@ size_t dc_window_bwd_workspace_size(const dc_window_desc *d) {
 }
 
 dc_status dc_window_bwd(const dc_window_desc *d, const void *grad_out, const void *q, const void *k,
-                        const void *v, const void *out, const float *lse, void *dq, void *dk, void *dv,
+                        const void *v, const void *out, const void *rest, const float *lse, void *dq, void *dk, void *dv,
                         void *workspace, size_t workspace_bytes, void *stream) {
     dc::WinArgs a;
     dc_status st = window_args(d, &a);
@@ -1023,10 +1023,11 @@ dc_status dc_window_bwd(const dc_window_desc *d, const void *grad_out, const voi
     if (nq > 0 && (workspace == nullptr || workspace_bytes < dc_window_bwd_workspace_size(d)))
         return fail(DC_INVALID_ARGUMENT, "window attention backward workspace is too small");
     a.dout = grad_out, a.q = q, a.k = k, a.v = v, a.out_in = out, a.lse_in = lse;
+    a.rest = const_cast<void *>(rest);  // read alone
     a.dq = dq, a.dk = dk, a.dv = dv;
     a.dsum = static_cast<float *>(workspace);
     a.kv_part = a.dsum ? a.dsum + window_dsum_ws(a) / sizeof(float) : nullptr;
-    a.vec = window_pieces(d, {grad_out, q, k, v, out, dq, dk, dv}, {a.qs, a.ks, a.vs, a.gs});
+    a.vec = window_pieces(d, {grad_out, q, k, v, out, rest, dq, dk, dv}, {a.qs, a.ks, a.vs, a.gs});
     return launched(dc::launch_window_bwd(a, d->dtype == DC_BF16, static_cast<hipStream_t>(stream)));
 }
 

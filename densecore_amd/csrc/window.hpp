@@ -2,10 +2,12 @@
 // forward and backward kernels share: which key tiles a block of queries reads, operand fragments of
 // both types and tiles of rows in LDS.
 //
-// One source for both types.  bf16 operands enter the MFMAs as they are, and what the kernels compute
-// (P, dS) as two bf16 terms hi + lo, carried to 2^-17.  float32 operands are split exactly into three
-// bf16 parts (x3.hpp), six products each, error below the float32 MFMA's.  So neither type has a
-// rounding to fewer bits before the result's own.
+// One source for both types.  float32 operands are split exactly into three bf16 parts (x3.hpp), six
+// products each, error below the float32 MFMA's.  bf16 operands enter the MFMAs as they are, and what the
+// kernels compute (P, dS) as two bf16 terms hi + lo, carried to 2^-17.  So neither type has a rounding to
+// fewer bits before the result's own.  (bf16 without the lo terms wherever every P of a block is below
+// 1/32: a training step of B2 H32/8 L8192 E128 W1024 takes 1738 us and not 1999, but its gradients are
+// 2.2e-3 from float64 by norm and not 1.7e-3, which is the rounding of the results alone.)
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -25,6 +27,7 @@ struct WinArgs {
     const float *lse_in;
     int64_t qs[3], ks[3], vs[3], gs[3];  // strides: batch, head, row
     void *out;
+    void *rest;           // bf16, optional: what rounding out left, itself rounded (forward: written, backward: read)
     float *lse;
     void *dq, *dk, *dv;
     float *dsum;          // (B, H, L): rowsum(dO * O)
@@ -65,6 +68,24 @@ namespace {
 // Whether the query at position p sees key s (s < S is the caller's).
 DEVI bool sees(int p, int s, int window, int sinks) { return s <= p && (p - s < window || s < sinks); }
 
+// Which of the keys base + c a query at p sees (c a constant): three compares, no branch.
+struct SeenKeys {
+    int hi, lo, sink;
+    DEVI SeenKeys(int p, int base, int S, int window, int sinks)
+        : hi(min(p, S - 1) - base), lo(max(p - window, -1) - base), sink(sinks - base) {}
+    DEVI bool operator()(int c) const { return (c <= hi) & ((c > lo) | (c < sink)); }
+};
+// And which of the queries at base + c see a key.
+struct SeenBy {
+    int first, end;
+    DEVI SeenBy(int key, int base, int S, int window, int sinks) : first(key < S ? key - base : 64) {
+        const int64_t e = (int64_t)key + window - base;
+        end = key < sinks || e > 64 ? 64 : (int)max(e, (int64_t)-64);
+    }
+    DEVI bool operator()(int c) const { return (c >= first) & (c < end); }
+};
+constexpr int acc_const(int e) { return 8 * (e >> 2) + (e & 3); }  // acc_row without its 4 g
+
 // The key tiles (of BN keys) that queries at positions p0 .. p1 read: ns tiles from key 0 (sinks), then
 // those from tile tb; n in all.  One run from tile 0 where the two meet.
 struct Band {
@@ -93,9 +114,6 @@ struct Ops;
 template <>
 struct Ops<__bf16> {
     typedef bf16x8 Frag;
-    struct PFrag {
-        bf16x8 h, l;
-    };
     template <int R, int D>
     struct Tile {
         u32x4 p[CMTile<R, D>::SLOTS];
@@ -106,19 +124,15 @@ struct Ops<__bf16> {
     DEVI static Frag tr(const Tile<R, D> &t, uint32_t base, int row0, int dt) { return tr_frag<R, D>(t.p, base, row0, dt); }
     static constexpr int READS = 1, MMAS = 1;  // 16-byte LDS reads of a row fragment, MFMAs of a product
     DEVI static f32x16 mma(Frag a, Frag b, f32x16 c) { return mfma_bf16(a, b, c); }
-    DEVI static PFrag split(const f32x16 &x, int at) {
-        PFrag p;
-        split_bf16(x, at, p.h, p.l);
-        return p;
-    }
-    // c[i] += a[i] p, the N independent chains product by product.
-    static constexpr int PRODUCTS = 2;
+    // c[i] += a[i] x[at .. at + 7], the N independent chains product by product.
     template <int N>
-    DEVI static void mma_p(const Frag (&a)[N], const PFrag &p, f32x16 (&c)[N]) {
+    DEVI static void mma_p(const Frag (&a)[N], const f32x16 &x, int at, f32x16 (&c)[N]) {
+        Frag h, l;
+        split_bf16(x, at, h, l);
 #pragma unroll
-        for (int i = 0; i < N; ++i) c[i] = mfma_bf16(a[i], p.l, c[i]);
+        for (int i = 0; i < N; ++i) c[i] = mfma_bf16(a[i], l, c[i]);
 #pragma unroll
-        for (int i = 0; i < N; ++i) c[i] = mfma_bf16(a[i], p.h, c[i]);
+        for (int i = 0; i < N; ++i) c[i] = mfma_bf16(a[i], h, c[i]);
     }
     // Dims d0 .. d0 + 7 of a row (0 past E, and all 0 without `in`).
     template <bool VEC>
@@ -149,7 +163,6 @@ struct Ops<__bf16> {
 template <>
 struct Ops<float> {
     typedef X3 Frag;
-    typedef X3 PFrag;
     template <int R, int D>
     using Tile = X3Tile<R, D>;
     template <int R, int D>
@@ -158,10 +171,9 @@ struct Ops<float> {
     DEVI static Frag tr(const Tile<R, D> &t, uint32_t base, int row0, int dt) { return tr_frag_x3<R, D>(t, base, row0, dt); }
     static constexpr int READS = 3, MMAS = 6;
     DEVI static f32x16 mma(const Frag &a, const Frag &b, f32x16 c) { return mfma_x3(a, b, c); }
-    DEVI static PFrag split(const f32x16 &x, int at) { return split3(x, at); }
-    static constexpr int PRODUCTS = 6;
     template <int N>
-    DEVI static void mma_p(const Frag (&a)[N], const PFrag &p, f32x16 (&c)[N]) {
+    DEVI static void mma_p(const Frag (&a)[N], const f32x16 &x, int at, f32x16 (&c)[N]) {
+        const X3 p = split3(x, at);
 #pragma unroll
         for (int j = 0; j < 6; ++j)
 #pragma unroll
@@ -290,6 +302,9 @@ DEVI void store4(T *row, int d, int E, float x0, float x1, float x2, float x3) {
             if (d + u < E) row[d + u] = from_f32<T>(x[u]);
     }
 }
+
+// What rounding x to bf16 leaves.
+DEVI float rest_of(float x) { return x - bf16_to_f32(f32_to_bf16(x)); }
 
 // a . b over E dims in plain float32, for rows computed again.
 template <typename T>

@@ -24,9 +24,12 @@ constexpr int kWavesPerSimd = sizeof(T) == 2 || D <= 64 ? 2 : 1;
 // dK / dV: waves w and w + 4 own the same 32 keys and halve each step's queries (one wave per SIMD: no halves).
 template <typename T, int D>
 constexpr int kHalves = kWavesPerSimd<T, D>;
-// dK / dV: K's and V's operands in LDS and not in registers (bf16 at D = 128, where the sums take half of them).
+// dK / dV: K's, V's operands in LDS and not in registers, where these would spill (at D = 128 the sums alone
+// take half of bf16's, and float32's take 350 with one wave per SIMD).
 template <typename T, int D>
-constexpr bool kKvLds = sizeof(T) == 2 && D == 128;
+constexpr bool kKLds = sizeof(T) == 2 && D == 128;
+template <typename T, int D>
+constexpr bool kVLds = D >= 64 && (sizeof(T) == 2 ? D == 128 : D == 64);
 
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(kThreads)
@@ -54,6 +57,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
     const T *qb = static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1];
     const T *gb = static_cast<const T *>(a.dout) + b * a.gs[0] + h * a.gs[1];
     const T *ob = static_cast<const T *>(a.out_in) + (int64_t)bh * a.L * a.E;
+    const T *rb = static_cast<const T *>(a.rest) + (int64_t)bh * a.L * a.E;
 
     typename O::Frag qf[KSTEP], gf[KSTEP];
     float dsum = 0.f;
@@ -62,6 +66,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
         qf[t] = O::template load<VEC>(qb + l * a.qs[2], 16 * t + 8 * g, a.E, in);
         gf[t] = O::template load<VEC>(gb + l * a.gs[2], 16 * t + 8 * g, a.E, in);
         dsum += O::dot(gf[t], O::template load<VEC>(ob + (int64_t)l * a.E, 16 * t + 8 * g, a.E, in));
+        if (sizeof(T) == 2 && a.rest) dsum += O::dot(gf[t], O::template load<VEC>(rb + (int64_t)l * a.E, 16 * t + 8 * g, a.E, in));
     }
     dsum = xor32_add(dsum);
     if (in && g == 0) a.dsum[row] = dsum;
@@ -114,19 +119,21 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
             load_k(0);
             if (all) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = exp2_fast(fmaf(s[e], a.scale_log2, nlse)) * t[e];
+                for (int e = 0; e < 16; ++e) s[e] = exp2_fast(fmaf(s[e], a.scale_log2, nlse));
             } else {
+                const SeenKeys seen(p, k0 + 4 * g, a.S, a.window, a.sinks);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = k0 + acc_row(e, g);
-                    const float ds = exp2_fast(fmaf(s[e], a.scale_log2, nlse)) * t[e];
-                    s[e] = key < a.S && sees(p, key, a.window, a.sinks) ? ds : 0.f;
-                }
+                for (int e = 0; e < 16; ++e) s[e] = exp2_fast(seen(acc_const(e)) ? fmaf(s[e], a.scale_log2, nlse) : -INFINITY);
             }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] *= t[e];
             if (sizeof(T) == 2) load_k(1);
-            O::mma_p(kf[0], O::split(s, 0), acc);
+            O::mma_p(kf[0], s, 0, acc);
             if (sizeof(T) != 2) load_k(1);
-            O::mma_p(kf[1], O::split(s, 8), acc);
+            O::mma_p(kf[1], s, 8, acc);
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) pin(acc[dt]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     for (int i = 0; i < band.n; ++i) {
@@ -155,7 +162,9 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
         const int rl = wr0 + __builtin_ctz(again), rp = a.offset + rl;
         const int64_t rr = (int64_t)bh * a.L + rl;
         const T *q1 = qb + rl * a.qs[2], *g1 = gb + rl * a.gs[2];
-        const float rs = plain_dot<T>(g1, ob + (int64_t)rl * a.E, a.E), rlse = a.lse_in[rr];
+        float rs = plain_dot<T>(g1, ob + (int64_t)rl * a.E, a.E);
+        if (sizeof(T) == 2 && a.rest) rs += plain_dot<T>(g1, rb + (int64_t)rl * a.E, a.E);
+        const float rlse = a.lse_in[rr];
         if (lane == 0) a.dsum[rr] = rs;
         float o[2] = {0.f, 0.f};
         for (int i = 0; i < band.n; ++i) {
@@ -211,13 +220,13 @@ __global__ __launch_bounds__((kThreads * kHalves<T, D>))
 __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) void window_dkdv_kernel(WinArgs a) {
     typedef Ops<T> O;
     constexpr int HALVES = kHalves<T, D>, QM = 32 * HALVES, THREADS = kThreads * HALVES, KSTEP = D / 16, NDT = D / 32;
-    constexpr bool KVLDS = kKvLds<T, D>;
+    constexpr bool KLDS = kKLds<T, D>, VLDS = kVLds<T, D>;
     typedef Stage<T, QM, D, THREADS, VEC> St;
-    typedef Stage<T, KVLDS ? kM : 32, D, THREADS, VEC> StV;
+    typedef Stage<T, VLDS ? kM : 32, D, THREADS, VEC> StV;
     struct Main {
         typename St::Tile q[2], g[2];
         float lse[2][QM], dsum[2][QM];  // -lse log2 e (-inf behind the last row: P = 0) and -dsum
-        typename StV::Tile k[KVLDS ? 1 : 0], v[KVLDS ? 1 : 0];
+        typename StV::Tile k[KLDS ? 1 : 0], v[VLDS ? 1 : 0];
     };
     union Smem {
         Main m;
@@ -273,25 +282,23 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
     };
 #pragma unroll
     for (int i = 0; i < 2; ++i) St::clear(sm.m.q[i], a.E, tid), St::clear(sm.m.g[i], a.E, tid);
-    if constexpr (KVLDS) {
-        StV kst, vst;
-        StV::clear(sm.m.k[0], a.E, tid), StV::clear(sm.m.v[0], a.E, tid);
-        kst.start(sm.m.k[0], kb + (int64_t)n0 * a.ks[2], a.ks[2], min(kM, a.S - n0), a.E, tid);
-        kst.finish(sm.m.k[0], tid);
-        vst.start(sm.m.v[0], vb + (int64_t)n0 * a.vs[2], a.vs[2], min(kM, a.S - n0), a.E, tid);
-        vst.finish(sm.m.v[0], tid);
-    }
+    auto hold = [&](auto &tile, const T *src, int64_t ld) {
+        StV x;
+        StV::clear(tile, a.E, tid);
+        x.start(tile, src + n0 * ld, ld, min(kM, a.S - n0), a.E, tid);
+        x.finish(tile, tid);
+    };
+    if constexpr (KLDS) hold(sm.m.k[0], kb, a.ks[2]);
+    if constexpr (VLDS) hold(sm.m.v[0], vb, a.vs[2]);
     At now = {0, 0};
     if (i0 < i1) now = first(i0), start(i0, now), finish(i0, now);
 
-    typename O::Frag kf[KVLDS ? 1 : KSTEP], vf[KVLDS ? 1 : KSTEP];
-    if constexpr (!KVLDS) {
+    typename O::Frag kf[KLDS ? 1 : KSTEP], vf[VLDS ? 1 : KSTEP];
 #pragma unroll
-        for (int t = 0; t < KSTEP; ++t) {
-            const int kr = min(key, a.S - 1);
-            kf[t] = O::template load<VEC>(kb + kr * a.ks[2], 16 * t + 8 * g, a.E, key < a.S);
-            vf[t] = O::template load<VEC>(vb + kr * a.vs[2], 16 * t + 8 * g, a.E, key < a.S);
-        }
+    for (int t = 0; t < KSTEP; ++t) {
+        const int kr = min(key, a.S - 1);
+        if constexpr (!KLDS) kf[t] = O::template load<VEC>(kb + kr * a.ks[2], 16 * t + 8 * g, a.E, key < a.S);
+        if constexpr (!VLDS) vf[t] = O::template load<VEC>(vb + kr * a.vs[2], 16 * t + 8 * g, a.E, key < a.S);
     }
     f32x16 dk[NDT], dv[NDT];
 #pragma unroll
@@ -299,7 +306,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[dt][e] = dv[dt][e] = 0.f;
     const uint32_t rowb = row_lanebase<QM, D>(lane), trb = tr_lanebase<QM, D>(lane);
-    const uint32_t rowk = row_lanebase<KVLDS ? kM : 32, D>(lane);
+    const uint32_t rowk = row_lanebase<VLDS ? kM : 32, D>(lane);
 
     auto step = [&](int i, At x) {
         const int buf = i & 1, mq = x.m + 32 * half, r0 = 32 * half;
@@ -316,24 +323,22 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int st = 0; st < KSTEP; ++st) {
-            if constexpr (KVLDS) {
-                s = O::mma(O::row(sm.m.q[buf], rowb, r0, st), O::row(sm.m.k[0], rowk, 32 * kw, st), s);
-                t = O::mma(O::row(sm.m.g[buf], rowb, r0, st), O::row(sm.m.v[0], rowk, 32 * kw, st), t);
-            } else {
-                s = O::mma(O::row(sm.m.q[buf], rowb, r0, st), kf[st], s);
-                t = O::mma(O::row(sm.m.g[buf], rowb, r0, st), vf[st], t);
-            }
+            if constexpr (KLDS) s = O::mma(O::row(sm.m.q[buf], rowb, r0, st), O::row(sm.m.k[0], rowk, 32 * kw, st), s);
+            else s = O::mma(O::row(sm.m.q[buf], rowb, r0, st), kf[st], s);
+            if constexpr (VLDS) t = O::mma(O::row(sm.m.g[buf], rowb, r0, st), O::row(sm.m.v[0], rowk, 32 * kw, st), t);
+            else t = O::mma(O::row(sm.m.g[buf], rowb, r0, st), vf[st], t);
         }
-        reads_ahead<KSTEP, 2 * O::MMAS, (KVLDS ? 4 : 2) * O::READS, sizeof(T) == 2 ? 2 : 1>();
+        reads_ahead<KSTEP, 2 * O::MMAS, (2 + KLDS + VLDS) * O::READS, sizeof(T) == 2 ? 2 : 1>();
         pin(s), pin(t);
         __builtin_amdgcn_sched_barrier(0);
         // dV^T += dO^T P and dK^T += Q^T dS, 16 queries at a time; bf16's transposed operands are read a
         // product ahead, the first while P and dS are formed.
-        typename O::Frag f[2][NDT];
+        constexpr int FB = sizeof(T) == 2 ? 2 : 1;
+        typename O::Frag f[FB][NDT];
         auto load = [&](int n) {
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt)
-                f[n & 1][dt] = O::tr((n & 1) ? sm.m.q[buf] : sm.m.g[buf], trb, r0 + 16 * (n >> 1), dt);
+                f[n % FB][dt] = O::tr((n & 1) ? sm.m.q[buf] : sm.m.g[buf], trb, r0 + 16 * (n >> 1), dt);
         };
         f32x4 nl[4];
 #pragma unroll
@@ -346,19 +351,18 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
                 t[e] *= s[e];
             }
         } else {
+            const SeenBy seen(key, q0 + 4 * g, a.S, a.window, a.sinks);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const bool seen = key < a.S && sees(q0 + acc_row(e, g), key, a.window, a.sinks);
-                const float pr = exp2_fast(fmaf(s[e], a.scale_log2, nl[e >> 2][e & 3]));
-                s[e] = seen ? pr : 0.f;
-                t[e] = seen ? pr * t[e] : 0.f;
+                s[e] = exp2_fast(seen(acc_const(e)) ? fmaf(s[e], a.scale_log2, nl[e >> 2][e & 3]) : -INFINITY);
+                t[e] *= s[e];
             }
         }
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             if (sizeof(T) == 2 && n + 1 < 4) load(n + 1);
-            if (n & 1) O::mma_p(f[n & 1], O::split(t, 8 * (n >> 1)), dk);
-            else O::mma_p(f[n & 1], O::split(s, 8 * (n >> 1)), dv);
+            if (n & 1) O::mma_p(f[n % FB], t, 8 * (n >> 1), dk);
+            else O::mma_p(f[n % FB], s, 8 * (n >> 1), dv);
             if (sizeof(T) != 2 && n + 1 < 4) load(n + 1);
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) pin((n & 1) ? dk[dt] : dv[dt]);

@@ -37,6 +37,13 @@ DEVI void positions(const WinArgs &a, int r0, int r1, int &p0, int &p1) {
     }
 }
 
+// Element i of the result.
+template <typename T>
+DEVI void put(const WinArgs &a, int64_t i, float x) {
+    static_cast<T *>(a.out)[i] = from_f32<T>(x);
+    if (sizeof(T) == 2 && a.rest) static_cast<T *>(a.rest)[i] = from_f32<T>(rest_of(x));
+}
+
 // One row again, keys of tiles [i0, i1): lanes are keys for the scores and dims for the output
 // (dims lane and lane + 64).  The maximum and sum first, so that the output is a sum of P / sum times v and
 // does not overflow where the result does not.
@@ -171,12 +178,12 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
         const bool all = n0 + BN <= a.S && n0 + BN - 1 <= wp0 && (wp1 - n0 < a.window || n0 + BN <= a.sinks);
         if (!all) {
 #pragma unroll
-            for (int kt = 0; kt < NT; ++kt)
+            for (int kt = 0; kt < NT; ++kt) {
+                // (A sub-tile that is not live holds no product: all of it is hidden.)
+                const SeenKeys seen(p, n0 + 32 * kt + 4 * g, a.S, a.window, a.sinks);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = n0 + 32 * kt + acc_row(e, g);
-                    if (!live[kt] || key >= a.S || !sees(p, key, a.window, a.sinks)) s[kt][e] = -INFINITY;
-                }
+                for (int e = 0; e < 16; ++e) s[kt][e] = seen(acc_const(e)) ? s[kt][e] : -INFINITY;
+            }
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -197,19 +204,21 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
         }
         const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
 #pragma unroll
-        for (int kt = 0; kt < NT; ++kt) {
+        for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 s[kt][e] = exp2_fast(fmaf(s[kt][e], c, neg_m));
                 l_part += s[kt][e];
             }
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt) {
             if (!live[kt]) continue;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 typename O::Frag vf[NDT];
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt) vf[dt] = O::tr(sv[buf], trb, 32 * kt + 16 * u, dt);
-                O::mma_p(vf, O::split(s[kt], 8 * u), acc);
+                O::mma_p(vf, s[kt], 8 * u, acc);
             }
         }
     };
@@ -244,9 +253,15 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    store4<T, VEC>(static_cast<T *>(a.out) + row * a.E, dt * 32 + acc_row(e, g), a.E, acc[dt][e] * inv,
-                                   acc[dt][e + 1] * inv, acc[dt][e + 2] * inv, acc[dt][e + 3] * inv);
+                for (int e = 0; e < 16; e += 4) {
+                    const int d = dt * 32 + acc_row(e, g);
+                    const float x0 = acc[dt][e] * inv, x1 = acc[dt][e + 1] * inv, x2 = acc[dt][e + 2] * inv,
+                                x3 = acc[dt][e + 3] * inv;
+                    store4<T, VEC>(static_cast<T *>(a.out) + row * a.E, d, a.E, x0, x1, x2, x3);
+                    if (sizeof(T) == 2 && a.rest)
+                        store4<T, VEC>(static_cast<T *>(a.rest) + row * a.E, d, a.E, rest_of(x0), rest_of(x1), rest_of(x2),
+                                       rest_of(x3));
+                }
             if (g == 0) a.lse[row] = empty ? 0.f : lse;
         }
     }
@@ -264,7 +279,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
         for (int d = lane, j = 0; j < 2; ++j, d += 64) {
             if (d >= a.E) continue;
             if (a.splits > 1) a.part[slot * a.E + d] = o[j];
-            else static_cast<T *>(a.out)[orow * a.E + d] = from_f32<T>(o[j]);
+            else put<T>(a, orow * a.E + d, o[j]);
         }
         if (lane == 0) {
             if (a.splits > 1) a.part_lse[slot] = none ? -INFINITY : lse;
@@ -289,7 +304,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinArgs a) {
         float o = 0.f;
         for (int i = 0; i < a.splits; ++i)
             o = fmaf(exp2_fast((a.part_lse[i * nrows + row] - base) * kLog2e) * inv, a.part[(i * nrows + row) * a.E + d], o);
-        static_cast<T *>(a.out)[row * a.E + d] = from_f32<T>(o);
+        put<T>(a, row * a.E + d, o);
     }
     if (part == 0) a.lse[row] = empty ? 0.f : base + log2_fast(sum) * kLn2;
 }

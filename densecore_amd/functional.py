@@ -307,8 +307,8 @@ def _window_numbers(window, sinks, offset, scale):
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, offset, scale):
-        out, lse = _native._window_attention(q, k, v, window, sinks, offset, scale)
-        ctx.save_for_backward(q, k, v, out, lse)
+        out, lse, rest = _native._window_attention(q, k, v, window, sinks, offset, scale, with_rest=True)
+        ctx.save_for_backward(q, k, v, out, lse, rest)
         ctx.args = (window, sinks, offset, scale)
         return out
 

@@ -45,16 +45,19 @@ typedef struct {
 #define DC_WINDOW_MAX_HEAD_DIM 128
 #define DC_WINDOW_DECODE_MAX_HEAD_DIM 256
 
-/* (out, lse).  The workspace is optional: it holds the partial results of key ranges that few rows
- * are split into. */
+/* (out, lse).  `rest` is optional and used for bfloat16: a tensor like out that takes what rounding out
+ * left, itself rounded.  dc_window_bwd forms rowsum(grad_out * out) from both; from the rounded out alone
+ * that sum is off by 2^-9 of its terms, which is most of dq where a query sees one key or nearly
+ * attends to one.  The workspace is optional: it holds the partial results of key ranges that few rows are
+ * split into. */
 size_t dc_window_fwd_workspace_size(const dc_window_desc *d);
 dc_status dc_window_fwd(const dc_window_desc *d, const void *q, const void *k, const void *v, void *out,
-                        float *lse, void *workspace, size_t workspace_bytes, void *stream);
+                        void *rest, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 
-/* (dq, dk, dv) from the saved out and lse.  The workspace is required. */
+/* (dq, dk, dv) from the saved out, rest (or NULL) and lse.  The workspace is required. */
 size_t dc_window_bwd_workspace_size(const dc_window_desc *d);
 dc_status dc_window_bwd(const dc_window_desc *d, const void *grad_out, const void *q, const void *k,
-                        const void *v, const void *out, const float *lse, void *dq, void *dk, void *dv,
+                        const void *v, const void *out, const void *rest, const float *lse, void *dq, void *dk, void *dv,
                         void *workspace, size_t workspace_bytes, void *stream);
 
 /* One query per sequence (q_len == 1; offset is not used) over a cache of kv_len rows of which sequence

@@ -252,6 +252,19 @@ def test_gradient_against_differences(dtype):
     assert abs(got - want) <= slack + 1e-6
 
 
+def test_rows_that_see_one_key_have_no_query_gradient():
+    """Softmax over one key is 1 whatever the query: dq is 0 but for float32's rounding of terms of size
+    |dO| |V|, also where the output was rounded to bf16 (2^-16 with its rest)."""
+    from densecore_amd import functional as F
+    gen = torch.Generator().manual_seed(16)
+    for dtype, u in ((torch.float32, U), (torch.bfloat16, 2.0 ** -16)):
+        q, k, v, g = (torch.randn(1, 2, 100, 64, generator=gen).to(dtype).to(DEV) for _ in range(4))
+        leaves = [t.requires_grad_(True) for t in (q, k, v)]
+        dq = torch.autograd.grad(F.window_attention(*leaves, 1), leaves, g)[0]
+        size = (g.double().abs() * v.detach().double().abs()).sum(-1, keepdim=True) * k.detach().double().abs() / 8
+        assert (dq.double().abs() <= (64 + 8) * U * size + u * size).all()
+
+
 @TYPES
 def test_rows_behind_the_results_are_left_alone(dtype):
     """Outputs, gradients and workspaces in the middle of larger buffers."""
@@ -273,8 +286,8 @@ def test_rows_behind_the_results_are_left_alone(dtype):
     def at(t):
         return t.data_ptr() + pad * t.element_size()
     st = _native._stream(q.device)
-    _lib.check(L_.dc_window_fwd(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), at(out), at(lse), at(ws[0]), fw, st))
-    _lib.check(L_.dc_window_bwd(d, g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), at(out), at(lse),
+    _lib.check(L_.dc_window_fwd(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), at(out), None, at(lse), at(ws[0]), fw, st))
+    _lib.check(L_.dc_window_bwd(d, g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), at(out), None, at(lse),
                                 *(at(t) for t in grads), at(ws[1]), bw, st))
     torch.cuda.synchronize()
     for t in (out, lse, *grads, *ws):

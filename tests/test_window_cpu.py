@@ -62,25 +62,25 @@ def _desc(**kw):
 ])
 def test_c_entries_refuse(kw, status):
     L, d = _lib.lib(), _desc(**kw)
-    assert L.dc_window_fwd(d, P, P, P, P, P, None, 0, None) == status
-    assert L.dc_window_bwd(d, *[P] * 10, 1 << 40, None) == status
+    assert L.dc_window_fwd(d, P, P, P, P, None, P, None, 0, None) == status
+    assert L.dc_window_bwd(d, *[P] * 11, 1 << 40, None) == status
     assert L.dc_window_decode(d, P, P, P, None, 0, P, P, P, 1 << 40, None) == status
     assert L.dc_last_error()
 
 
 def test_c_entries_refuse_pointers_and_workspaces():
     L, bad = _lib.lib(), _lib.DC_INVALID_ARGUMENT
-    assert L.dc_window_fwd(None, P, P, P, P, P, None, 0, None) == bad
-    assert L.dc_window_fwd(_desc(), P, None, P, P, P, None, 0, None) == bad
-    assert L.dc_window_fwd(_desc(), P, P, P, P, None, None, 0, None) == bad
-    assert L.dc_window_fwd(_desc(head_dim=129), P, P, P, P, P, None, 0, None) == _lib.DC_UNSUPPORTED
+    assert L.dc_window_fwd(None, P, P, P, P, None, P, None, 0, None) == bad
+    assert L.dc_window_fwd(_desc(), P, None, P, P, None, P, None, 0, None) == bad
+    assert L.dc_window_fwd(_desc(), P, P, P, P, None, None, None, 0, None) == bad
+    assert L.dc_window_fwd(_desc(head_dim=129), P, P, P, P, None, P, None, 0, None) == _lib.DC_UNSUPPORTED
     size = L.dc_window_bwd_workspace_size(_desc())
     assert size > 0
-    assert L.dc_window_bwd(_desc(), *[P] * 9, None, size, None) == bad
-    assert L.dc_window_bwd(_desc(), *[P] * 10, size - 1, None) == bad
+    assert L.dc_window_bwd(_desc(), *[P] * 10, None, size, None) == bad
+    assert L.dc_window_bwd(_desc(), *[P] * 11, size - 1, None) == bad
     assert L.dc_window_decode(_desc(q_len=2), P, P, P, None, 0, P, P, P, 1 << 40, None) == bad
     assert L.dc_window_decode(_desc(), P, P, P, P, 2, P, P, P, 1 << 40, None) == bad
     assert L.dc_window_decode(_desc(), P, P, P, None, 8, P, P, P, 1 << 40, None) == bad
     # Nothing to compute: no pointer is looked at.
-    assert L.dc_window_fwd(_desc(batch=0), *[None] * 6, 0, None) == _lib.DC_OK
+    assert L.dc_window_fwd(_desc(batch=0), *[None] * 7, 0, None) == _lib.DC_OK
     assert L.dc_window_decode(_desc(batch=0), None, None, None, None, 0, None, None, None, 0, None) == _lib.DC_OK
