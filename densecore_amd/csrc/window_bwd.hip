@@ -59,6 +59,21 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
     const T *ob = static_cast<const T *>(a.out_in) + (int64_t)bh * a.L * a.E;
     const T *rb = static_cast<const T *>(a.rest) + (int64_t)bh * a.L * a.E;
 
+    const uint32_t rowb = row_lanebase<BN, D>(lane), trb = tr_lanebase<BN, D>(lane);
+    St kst, vst;
+    auto start = [&](int i) {
+        const int n0 = band.tile(i) * BN, nr = min(BN, a.S - n0);
+        kst.start(sk[i & 1], kb + (int64_t)n0 * a.ks[2], a.ks[2], nr, a.E, tid);
+        vst.start(sv[i & 1], vb + (int64_t)n0 * a.vs[2], a.vs[2], nr, a.E, tid);
+    };
+    auto finish = [&](int i) {
+        kst.finish(sk[i & 1], tid);
+        vst.finish(sv[i & 1], tid);
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) St::clear(sk[i], a.E, tid), St::clear(sv[i], a.E, tid);
+    if (band.n > 0) start(0);  // on its way while the queries load
+
     typename O::Frag qf[KSTEP], gf[KSTEP];
     float dsum = 0.f;
 #pragma unroll
@@ -78,20 +93,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
 
-    const uint32_t rowb = row_lanebase<BN, D>(lane), trb = tr_lanebase<BN, D>(lane);
-    St kst, vst;
-    auto start = [&](int i) {
-        const int n0 = band.tile(i) * BN, nr = min(BN, a.S - n0);
-        kst.start(sk[i & 1], kb + (int64_t)n0 * a.ks[2], a.ks[2], nr, a.E, tid);
-        vst.start(sv[i & 1], vb + (int64_t)n0 * a.vs[2], a.vs[2], nr, a.E, tid);
-    };
-    auto finish = [&](int i) {
-        kst.finish(sk[i & 1], tid);
-        vst.finish(sv[i & 1], tid);
-    };
-#pragma unroll
-    for (int i = 0; i < 2; ++i) St::clear(sk[i], a.E, tid), St::clear(sv[i], a.E, tid);
-    if (band.n > 0) start(0), finish(0);
+    if (band.n > 0) finish(0);
 
     auto step = [&](int i) {
         const int n0 = band.tile(i) * BN;
@@ -282,16 +284,17 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
     };
 #pragma unroll
     for (int i = 0; i < 2; ++i) St::clear(sm.m.q[i], a.E, tid), St::clear(sm.m.g[i], a.E, tid);
-    auto hold = [&](auto &tile, const T *src, int64_t ld) {
-        StV x;
+    auto hold = [&](StV &x, auto &tile, const T *src, int64_t ld) {
         StV::clear(tile, a.E, tid);
         x.start(tile, src + n0 * ld, ld, min(kM, a.S - n0), a.E, tid);
-        x.finish(tile, tid);
     };
-    if constexpr (KLDS) hold(sm.m.k[0], kb, a.ks[2]);
-    if constexpr (VLDS) hold(sm.m.v[0], vb, a.vs[2]);
+    StV kst, vst;
+    if constexpr (KLDS) hold(kst, sm.m.k[0], kb, a.ks[2]);
+    if constexpr (VLDS) hold(vst, sm.m.v[0], vb, a.vs[2]);
+    if constexpr (KLDS) kst.finish(sm.m.k[0], tid);
+    if constexpr (VLDS) vst.finish(sm.m.v[0], tid);
     At now = {0, 0};
-    if (i0 < i1) now = first(i0), start(i0, now), finish(i0, now);
+    if (i0 < i1) now = first(i0), start(i0, now);
 
     typename O::Frag kf[KLDS ? 1 : KSTEP], vf[VLDS ? 1 : KSTEP];
 #pragma unroll
@@ -300,6 +303,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
         if constexpr (!KLDS) kf[t] = O::template load<VEC>(kb + kr * a.ks[2], 16 * t + 8 * g, a.E, key < a.S);
         if constexpr (!VLDS) vf[t] = O::template load<VEC>(vb + kr * a.vs[2], 16 * t + 8 * g, a.E, key < a.S);
     }
+    if (i0 < i1) finish(i0, now);
     f32x16 dk[NDT], dv[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)

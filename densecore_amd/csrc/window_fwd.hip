@@ -78,6 +78,72 @@ DEVI void plain_row(const WinArgs &a, const T *q, const T *kb, const T *vb, int 
     }
 }
 
+// The end of a wave: O / sum and lse of its 32 rows (from row wr0 of the group on, this lane's `row` of out),
+// or the piece's share of them; rows that are not finite again.
+template <typename T, int D, bool VEC>
+DEVI void write_rows(const WinArgs &a, const f32x16 (&acc)[D / 32], float m_run, float l_part, int lane, int wr0, bool in,
+                     int64_t row, int b, int h0, const T *kb, const T *vb, Band band, int i0, int i1, int piece) {
+    constexpr int NDT = D / 32;
+    const int lr = lane & 31, g = lane >> 5;
+    const float l_run = xor32_add(l_part);
+    const bool empty = l_run == 0.f;
+    const float inv = empty ? 0.f : 1.f / l_run;
+    float test = l_run * 0.f;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) test += not_finite(acc[dt]);
+    const uint64_t wrong = __ballot(in && test != 0.f);
+    uint32_t again = (uint32_t)wrong | (uint32_t)(wrong >> 32);
+    const int64_t nrows = (int64_t)a.B * a.H * a.L;
+    if (in && !((again >> lr) & 1)) {
+        const float lse = (m_run + log2_fast(l_run)) * kLn2;
+        if (a.splits > 1) {
+            const int64_t slot = piece * nrows + row;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    store4<float, VEC>(a.part + slot * a.E, dt * 32 + acc_row(e, g), a.E, acc[dt][e] * inv, acc[dt][e + 1] * inv,
+                                       acc[dt][e + 2] * inv, acc[dt][e + 3] * inv);
+            if (g == 0) a.part_lse[slot] = empty ? -INFINITY : lse;
+        } else {
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const int d = dt * 32 + acc_row(e, g);
+                    const float x0 = acc[dt][e] * inv, x1 = acc[dt][e + 1] * inv, x2 = acc[dt][e + 2] * inv,
+                                x3 = acc[dt][e + 3] * inv;
+                    store4<T, VEC>(static_cast<T *>(a.out) + row * a.E, d, a.E, x0, x1, x2, x3);
+                    if (sizeof(T) == 2 && a.rest)
+                        store4<T, VEC>(static_cast<T *>(a.rest) + row * a.E, d, a.E, rest_of(x0), rest_of(x1), rest_of(x2),
+                                       rest_of(x3));
+                }
+            if (g == 0) a.lse[row] = empty ? 0.f : lse;
+        }
+    }
+    for (; again; again &= again - 1) {
+        const int rr = wr0 + __builtin_ctz(again);
+        const RowAt ra = row_at(a, rr);
+        const int64_t orow = ((int64_t)b * a.H + h0 + ra.h) * a.L + ra.l;
+        float o[2], m, sum;
+        plain_row<T>(a, static_cast<const T *>(a.q) + b * a.qs[0] + (h0 + ra.h) * a.qs[1] + ra.l * a.qs[2], kb, vb,
+                     a.offset + ra.l, band, i0, i1, lane, o, m, sum);
+        const bool none = sum == 0.f;
+        const float lse = (m + log2_fast(sum)) * kLn2;
+        const int64_t slot = piece * nrows + orow;
+#pragma unroll
+        for (int d = lane, j = 0; j < 2; ++j, d += 64) {
+            if (d >= a.E) continue;
+            if (a.splits > 1) a.part[slot * a.E + d] = o[j];
+            else put<T>(a, orow * a.E + d, o[j]);
+        }
+        if (lane == 0) {
+            if (a.splits > 1) a.part_lse[slot] = none ? -INFINITY : lse;
+            else a.lse[orow] = none ? 0.f : lse;
+        }
+    }
+}
+
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) void window_fwd_kernel(WinArgs a) {
@@ -111,6 +177,21 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
     const T *vb = static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1];
     const T *q = static_cast<const T *>(a.q) + b * a.qs[0] + (h0 + at.h) * a.qs[1] + at.l * a.qs[2];
 
+    const uint32_t rowb = row_lanebase<BN, D>(lane), trb = tr_lanebase<BN, D>(lane);
+    St kst, vst;
+    auto start = [&](int i) {
+        const int n0 = band.tile(i) * BN, nr = min(BN, a.S - n0), buf = (i - i0) & 1;
+        kst.start(sk[buf], kb + (int64_t)n0 * a.ks[2], a.ks[2], nr, a.E, tid);
+        vst.start(sv[buf], vb + (int64_t)n0 * a.vs[2], a.vs[2], nr, a.E, tid);
+    };
+    auto finish = [&](int i) {
+        kst.finish(sk[(i - i0) & 1], tid);
+        vst.finish(sv[(i - i0) & 1], tid);
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) St::clear(sk[i], a.E, tid), St::clear(sv[i], a.E, tid);
+    if (i0 < i1) start(i0);  // on its way while the queries load
+
     // Scores are fma(q.k, c, -m) in base 2; a negative scale is a sign flip of the queries, and a zero
     // one the smallest normal number (every visible key then gets P = 1).
     const float c = fmaxf(fabsf(a.scale_log2), 0x1p-126f);
@@ -127,20 +208,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
         for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
     float m_run = -INFINITY, l_part = 0.f;  // l_part: this half-wave's keys only
 
-    const uint32_t rowb = row_lanebase<BN, D>(lane), trb = tr_lanebase<BN, D>(lane);
-    St kst, vst;
-    auto start = [&](int i) {
-        const int n0 = band.tile(i) * BN, nr = min(BN, a.S - n0), buf = (i - i0) & 1;
-        kst.start(sk[buf], kb + (int64_t)n0 * a.ks[2], a.ks[2], nr, a.E, tid);
-        vst.start(sv[buf], vb + (int64_t)n0 * a.vs[2], a.vs[2], nr, a.E, tid);
-    };
-    auto finish = [&](int i) {
-        kst.finish(sk[(i - i0) & 1], tid);
-        vst.finish(sv[(i - i0) & 1], tid);
-    };
-#pragma unroll
-    for (int i = 0; i < 2; ++i) St::clear(sk[i], a.E, tid), St::clear(sv[i], a.E, tid);
-    if (i0 < i1) start(i0), finish(i0);
+    if (i0 < i1) finish(i0);
 
     auto step = [&](int i) {
         const int n0 = band.tile(i) * BN, buf = (i - i0) & 1;
@@ -229,63 +297,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
         if (i + 1 < i1) finish(i + 1);
     }
 
-    const float l_run = xor32_add(l_part);
-    const bool empty = l_run == 0.f;
-    const float inv = empty ? 0.f : 1.f / l_run;
-    float test = l_run * 0.f;
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) test += not_finite(acc[dt]);
-    const uint64_t wrong = __ballot(in && test != 0.f);
-    uint32_t again = (uint32_t)wrong | (uint32_t)(wrong >> 32);
-    const int64_t nrows = (int64_t)a.B * a.H * a.L;
-    if (in && !((again >> lr) & 1)) {
-        const float lse = (m_run + log2_fast(l_run)) * kLn2;
-        if (a.splits > 1) {
-            const int64_t slot = piece * nrows + row;
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    store4<float, VEC>(a.part + slot * a.E, dt * 32 + acc_row(e, g), a.E, acc[dt][e] * inv, acc[dt][e + 1] * inv,
-                                       acc[dt][e + 2] * inv, acc[dt][e + 3] * inv);
-            if (g == 0) a.part_lse[slot] = empty ? -INFINITY : lse;
-        } else {
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const int d = dt * 32 + acc_row(e, g);
-                    const float x0 = acc[dt][e] * inv, x1 = acc[dt][e + 1] * inv, x2 = acc[dt][e + 2] * inv,
-                                x3 = acc[dt][e + 3] * inv;
-                    store4<T, VEC>(static_cast<T *>(a.out) + row * a.E, d, a.E, x0, x1, x2, x3);
-                    if (sizeof(T) == 2 && a.rest)
-                        store4<T, VEC>(static_cast<T *>(a.rest) + row * a.E, d, a.E, rest_of(x0), rest_of(x1), rest_of(x2),
-                                       rest_of(x3));
-                }
-            if (g == 0) a.lse[row] = empty ? 0.f : lse;
-        }
-    }
-    for (; again; again &= again - 1) {
-        const int rr = wr0 + __builtin_ctz(again);
-        const RowAt ra = row_at(a, rr);
-        const int64_t orow = ((int64_t)b * a.H + h0 + ra.h) * a.L + ra.l;
-        float o[2], m, sum;
-        plain_row<T>(a, static_cast<const T *>(a.q) + b * a.qs[0] + (h0 + ra.h) * a.qs[1] + ra.l * a.qs[2], kb, vb,
-                     a.offset + ra.l, band, i0, i1, lane, o, m, sum);
-        const bool none = sum == 0.f;
-        const float lse = (m + log2_fast(sum)) * kLn2;
-        const int64_t slot = piece * nrows + orow;
-#pragma unroll
-        for (int d = lane, j = 0; j < 2; ++j, d += 64) {
-            if (d >= a.E) continue;
-            if (a.splits > 1) a.part[slot * a.E + d] = o[j];
-            else put<T>(a, orow * a.E + d, o[j]);
-        }
-        if (lane == 0) {
-            if (a.splits > 1) a.part_lse[slot] = none ? -INFINITY : lse;
-            else a.lse[orow] = none ? 0.f : lse;
-        }
-    }
+    write_rows<T, D, VEC>(a, acc, m_run, l_part, lane, wr0, in, row, b, h0, kb, vb, band, i0, i1, piece);
 }
 
 // Joins the pieces of each row, 16 lanes per row: lse = log sum exp(lse_i), out = sum exp(lse_i - lse) o_i.

@@ -115,6 +115,46 @@ def test_forward_and_gradients(case, dtype):
         close(d, *ref[name], dtype, name)
 
 
+MANY = [  # enough rows and heads to fill the device (other kernels, grids and pieces than a few heads take)
+    (16, 16, 4, 300, 300, 64, 100, 4, 0),
+    (16, 16, 16, 257, 257, 24, 1, 0, 0),
+    (9, 30, 10, 400, 400, 96, 130, 70, 0),
+    (8, 16, 2, 513, 700, 128, 300, 4, 187),
+    (8, 32, 32, 260, 130, 32, 64, 0, 3),
+    (4, 64, 64, 300, 300, 128, 4000, 0, 0),
+    (3, 8, 4, 1500, 1500, 80, 64, 4, 0),
+    (17, 16, 8, 290, 290, 100, 30, 200, 0),
+]
+
+
+@TYPES
+@pytest.mark.parametrize("case", MANY, ids=lambda c: "-".join(map(str, c)))
+def test_many_heads(case, dtype):
+    test_forward_and_gradients(case, dtype)
+
+
+@TYPES
+def test_many_heads_with_values_that_are_not_finite(dtype):
+    """As test_hidden_keys_have_no_influence, on a grid that fills the device."""
+    from densecore_amd import functional as F
+    gen = torch.Generator().manual_seed(17)
+    B, H, L, E, window = 8, 32, 300, 64, 50
+    q, k, v, g = (torch.randn(B, H, L, E, generator=gen).to(dtype).to(DEV) for _ in range(4))
+    ref = formulas(q, k, v, visible(torch.arange(L, device=DEV), L, window, 0), 1 / math.sqrt(E), dtype, g)
+    k2, v2 = k.clone(), v.clone()
+    k2[3, 7, 100], v2[3, 7, 100] = math.nan, math.inf
+    leaves = [t.requires_grad_(True) for t in (q, k2, v2)]
+    y = F.window_attention(*leaves, window)
+    hit = torch.zeros(B, H, L, dtype=torch.bool, device=DEV)
+    hit[3, 7, 100:100 + window] = True
+    assert torch.isnan(y[hit]).all()
+    near = torch.zeros_like(hit)
+    near[3, 7, 100 - window + 1:100 + window] = True
+    dq, dk, dv = torch.autograd.grad(y, leaves, g)
+    for name, d, m in (("out", y, hit), ("dq", dq, hit), ("dk", dk, near), ("dv", dv, near)):
+        close(d[~m], ref[name][0][~m], ref[name][1].expand_as(ref[name][0])[~m], dtype, name)
+
+
 @TYPES
 @pytest.mark.parametrize("scale", [0.0, -0.2, 1.5])
 def test_scales(scale, dtype):
