@@ -125,6 +125,26 @@ DEVI float xor32_add(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+template <int CTRL>
+DEVI float dpp_add(float x) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+// The sum over N neighbouring lanes (a power of two from 4), in all of them, without LDS: quads, then
+// quads of 8 and halves of 16 (mirrors within the row), 32 and 64.
+template <int N>
+DEVI float lanes_sum(float x) {
+    x = dpp_add<0xb1>(x);                   // quad_perm [1, 0, 3, 2]
+    x = dpp_add<0x4e>(x);                   // quad_perm [2, 3, 0, 1]
+    if (N >= 8) x = dpp_add<0x141>(x);      // row_half_mirror
+    if (N >= 16) x = dpp_add<0x140>(x);     // row_mirror
+    if (N >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if (N >= 64) x = xor32_add(x);
+    return x;
+}
+
 DEVI float bf16_to_f32(__bf16 x) { return static_cast<float>(x); }
 DEVI __bf16 f32_to_bf16(float x) { return static_cast<__bf16>(x); }  // round to nearest even
 

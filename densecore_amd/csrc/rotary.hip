@@ -44,18 +44,7 @@ DEVI void turn_of(double t, float m, float &c, float &s) {
     s = ((quad & 2) ? -b : b) * m;
 }
 
-// V consecutive values as float32, one load where V > 1 (the launcher checks the alignment).
-template <typename T, int V>
-DEVI void load_v(const T *p, float (&x)[V]) {
-    if constexpr (V == 1) {
-        x[0] = to_f32<T>(*p);
-    } else {
-        typedef T vec __attribute__((ext_vector_type(V)));
-        const vec r = *reinterpret_cast<const vec *>(p);
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = to_f32<T>(r[e]);
-    }
-}
+// V consecutive values, one store where V > 1 (the launcher checks the alignment).
 template <typename T, int V>
 DEVI void store_v(T *p, const float (&x)[V]) {
     if constexpr (V == 1) {
@@ -82,16 +71,29 @@ DEVI Unit unit_of(int u, int E, int R, bool interleaved) {
     return {R + t, min(R + rest + t, E), t < rest, false};
 }
 
-// One unit's values of a row: xa, xb.
+// A lane's pieces of a row as they lie (loads in flight cost no more registers than that), and as float32.
+template <typename T, int V, int NU>
+struct RowRaw {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    vec a[NU], b[NU];
+    // (Pieces a lane does not have are 0.)
+    DEVI void load(const T *row, const Unit (&un)[NU], int E, bool in) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const bool ina = in && un[i].in, inb = ina && (V > 1 || un[i].b < E);
+            a[i] = ina ? *reinterpret_cast<const vec *>(row + un[i].a) : vec(T(0));
+            b[i] = inb ? *reinterpret_cast<const vec *>(row + un[i].b) : vec(T(0));
+        }
+    }
+};
 template <typename T, int V, int NU>
 struct RowVals {
     float a[NU][V], b[NU][V];
-    DEVI void load(const T *row, const Unit (&un)[NU], int E) {
+    DEVI void set(const RowRaw<T, V, NU> &r) {
 #pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            if (un[i].in) load_v<T, V>(row + un[i].a, a[i]);
-            if (un[i].in && (V > 1 || un[i].b < E)) load_v<T, V>(row + un[i].b, b[i]);
-        }
+        for (int i = 0; i < NU; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) a[i][e] = to_f32<T>(r.a[i][e]), b[i][e] = to_f32<T>(r.b[i][e]);
     }
     DEVI void store(T *row, const Unit (&un)[NU], int E) const {
 #pragma unroll
@@ -100,26 +102,24 @@ struct RowVals {
             if (un[i].in && (V > 1 || un[i].b < E)) store_v<T, V>(row + un[i].b, b[i]);
         }
     }
-    DEVI void clear() {
-#pragma unroll
-        for (int i = 0; i < NU; ++i)
-#pragma unroll
-            for (int e = 0; e < V; ++e) a[i][e] = b[i][e] = 0.f;
-    }
 };
 
 // Cosines and sines of a lane's pairs (1 and 0 where the dims are not rotated).
 template <int V, int NU>
 struct Angles {
     float c[NU][V], s[NU][V];
-    DEVI void set(double p, const double (&f)[NU][V], const Unit (&un)[NU], float m) {
+    DEVI void set(double p, const RotArgs &a, int lane_u, int G, const Unit (&un)[NU]) {
+        typedef double vec __attribute__((ext_vector_type(V)));
+        p *= 0.63661977236758134;  // quarter turns
 #pragma unroll
-        for (int i = 0; i < NU; ++i)
+        for (int i = 0; i < NU; ++i) {
+            const vec f = un[i].turned ? *reinterpret_cast<const vec *>(a.freq + (lane_u + i * G) * V) : vec(0.0);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                c[i][e] = 1.f, s[i][e] = 0.f;
-                if (un[i].turned) turn_of(p * f[i][e], m, c[i][e], s[i][e]);
+                turn_of(p * f[e], a.magnitude, c[i][e], s[i][e]);
+                if (!un[i].turned) c[i][e] = 1.f, s[i][e] = 0.f;
             }
+        }
     }
     // The turn (sign 1) or the turn back (sign -1) of a row's values.
     template <typename T>
@@ -151,16 +151,6 @@ struct Angles {
     }
 };
 
-// Radian frequencies of a lane's pairs in quarter turns.
-template <int V, int NU>
-DEVI void load_freq(const RotArgs &a, int lane_u, int G, const Unit (&un)[NU], double (&f)[NU][V]) {
-#pragma unroll
-    for (int i = 0; i < NU; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            f[i][e] = un[i].turned ? a.freq[(lane_u + i * G) * V + e] * 0.63661977236758134 : 0.0;
-}
-
 DEVI double position_of(const RotArgs &a, int64_t b, int64_t l) {
     if (a.pos_bytes == 0) return (double)(a.offset + l);
     const int64_t at = b * a.pos_sb + l * a.pos_sl;
@@ -168,26 +158,23 @@ DEVI double position_of(const RotArgs &a, int64_t b, int64_t l) {
                             : (double)static_cast<const int32_t *>(a.pos)[at];
 }
 
-template <int V, int NU>
-DEVI void load_weight(const void *w, bool bf16, const Unit (&un)[NU], int E, float (&wa)[NU][V], float (&wb)[NU][V]) {
-    auto at = [&](int d) {
-        if (!w) return 1.f;
-        return bf16 ? bf16_to_f32(static_cast<const __bf16 *>(w)[d]) : static_cast<const float *>(w)[d];
-    };
+template <typename W, int V, int NU>
+DEVI void load_weight_of(const W *w, const Unit (&un)[NU], int E, float (&wa)[NU][V], float (&wb)[NU][V]) {
+    RowRaw<W, V, NU> raw;
+    raw.load(w, un, E, true);
 #pragma unroll
     for (int i = 0; i < NU; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            wa[i][e] = un[i].in ? at(un[i].a + e) : 0.f;
-            wb[i][e] = un[i].in && un[i].b + e < E ? at(un[i].b + e) : 0.f;
-        }
+        for (int e = 0; e < V; ++e) wa[i][e] = to_f32<W>(raw.a[i][e]), wb[i][e] = to_f32<W>(raw.b[i][e]);
 }
-
-template <int G>
-DEVI float group_sum(float x) {
+template <int V, int NU>
+DEVI void load_weight(const void *w, bool bf16, const Unit (&un)[NU], int E, float (&wa)[NU][V], float (&wb)[NU][V]) {
+    if (w && bf16) return load_weight_of<__bf16, V, NU>(static_cast<const __bf16 *>(w), un, E, wa, wb);
+    if (w) return load_weight_of<float, V, NU>(static_cast<const float *>(w), un, E, wa, wb);
 #pragma unroll
-    for (int o = 1; o < G; o <<= 1) x += __shfl_xor(x, o, 64);
-    return x;
+    for (int i = 0; i < NU; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) wa[i][e] = wb[i][e] = 1.f;
 }
 
 // Forward (and, with inverse and no norm, the gradient): items of (block of hb heads, token), token
@@ -199,11 +186,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotArgs a, bool invers
     const int64_t stride = (int64_t)gridDim.x * (kThreads / G);
     const int qb = (a.t[0].heads + a.hb - 1) / a.hb, kb = (a.t[1].heads + a.hb - 1) / a.hb;
     const int64_t items = (int64_t)(qb + kb) * a.tokens;
+    const float inv_e = 1.f / (float)a.E;
     Unit un[NU];
 #pragma unroll
     for (int i = 0; i < NU; ++i) un[i] = unit_of<V>(lane_u + i * G, a.E, a.R, a.interleaved);
-    double f[NU][V];
-    load_freq<V, NU>(a, lane_u, G, un, f);
     for (int64_t item = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G; item < items; item += stride) {
         const int64_t token = item % a.tokens;
         int blk = (int)(item / a.tokens);
@@ -217,35 +203,33 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotArgs a, bool invers
         src += b * sb + l * sl;
         T *dst = static_cast<T *>(t.out) + (b * t.heads * a.L + l) * a.E;
         Angles<V, NU> ang;
-        RowVals<T, V, NU> x[HU];
+        RowRaw<T, V, NU> raw[HU];
         float wa[NU][V], wb[NU][V];
         for (int h = h0; h < h1; h += HU) {
 #pragma unroll
-            for (int j = 0; j < HU; ++j) {
-                if constexpr (NORM) x[j].clear();
-                if (h + j < h1) x[j].load(src + (h + j) * sh, un, a.E);
-            }
+            for (int j = 0; j < HU; ++j) raw[j].load(src + (h + j) * sh, un, a.E, h + j < h1);
             if (h == h0) {  // while the first rows are on their way
-                ang.set(position_of(a, b, l), f, un, a.magnitude);
+                ang.set(position_of(a, b, l), a, lane_u, G, un);
                 if constexpr (NORM) load_weight<V, NU>(t.w, a.w_bf16, un, a.E, wa, wb);
             }
 #pragma unroll
             for (int j = 0; j < HU; ++j) {
+                RowVals<T, V, NU> x;
+                x.set(raw[j]);
                 if constexpr (NORM) {
                     float ss = 0.f;
 #pragma unroll
                     for (int i = 0; i < NU; ++i)
 #pragma unroll
-                        for (int e = 0; e < V; ++e) ss = fmaf(x[j].a[i][e], x[j].a[i][e], fmaf(x[j].b[i][e], x[j].b[i][e], ss));
-                    ss = group_sum<G>(ss);
-                    const float r = 1.f / sqrtf(ss / (float)a.E + a.eps);
+                        for (int e = 0; e < V; ++e) ss = fmaf(x.a[i][e], x.a[i][e], fmaf(x.b[i][e], x.b[i][e], ss));
+                    const float r = rsqrtf(fmaf(lanes_sum<G>(ss), inv_e, a.eps));
 #pragma unroll
                     for (int i = 0; i < NU; ++i)
 #pragma unroll
-                        for (int e = 0; e < V; ++e) x[j].a[i][e] *= r * wa[i][e], x[j].b[i][e] *= r * wb[i][e];
+                        for (int e = 0; e < V; ++e) x.a[i][e] *= r * wa[i][e], x.b[i][e] *= r * wb[i][e];
                 }
-                ang.apply(x[j], un, a.interleaved, inverse ? -1.f : 1.f);
-                if (h + j < h1) x[j].store(dst + (int64_t)(h + j) * a.L * a.E, un, a.E);
+                ang.apply(x, un, a.interleaved, inverse ? -1.f : 1.f);
+                if (h + j < h1) x.store(dst + (int64_t)(h + j) * a.L * a.E, un, a.E);
             }
         }
     }
@@ -266,11 +250,10 @@ __global__ __launch_bounds__(kThreads) void rotary_norm_bwd_kernel(RotArgs a) {
     const RotRows &t = a.t[which];
     const int64_t stride = (int64_t)a.nblk[which] * (kThreads / G);
     const int64_t items = (int64_t)((t.heads + a.hb - 1) / a.hb) * a.tokens;
+    const float inv_e = 1.f / (float)a.E;
     Unit un[NU];
 #pragma unroll
     for (int i = 0; i < NU; ++i) un[i] = unit_of<V>(lane_u + i * G, a.E, a.R, a.interleaved);
-    double f[NU][V];
-    load_freq<V, NU>(a, lane_u, G, un, f);
     float wa[NU][V], wb[NU][V], da[NU][V], db[NU][V];
     load_weight<V, NU>(t.w, a.w_bf16, un, a.E, wa, wb);
 #pragma unroll
@@ -285,42 +268,41 @@ __global__ __launch_bounds__(kThreads) void rotary_norm_bwd_kernel(RotArgs a) {
         const T *grd = static_cast<const T *>(t.g) + b * t.gs[0] + l * t.gs[2];
         T *dst = static_cast<T *>(t.out) + (b * t.heads * a.L + l) * a.E;
         Angles<V, NU> ang;
-        RowVals<T, V, NU> x[HU], y[HU];
+        RowRaw<T, V, NU> xr[HU], yr[HU];
         for (int h = h0; h < h1; h += HU) {
 #pragma unroll
             for (int j = 0; j < HU; ++j) {
-                x[j].clear(), y[j].clear();
-                if (h + j < h1) {
-                    x[j].load(src + (h + j) * t.xs[1], un, a.E);
-                    y[j].load(grd + (h + j) * t.gs[1], un, a.E);
-                }
+                xr[j].load(src + (h + j) * t.xs[1], un, a.E, h + j < h1);
+                yr[j].load(grd + (h + j) * t.gs[1], un, a.E, h + j < h1);
             }
-            if (h == h0) ang.set(position_of(a, b, l), f, un, a.magnitude);
+            if (h == h0) ang.set(position_of(a, b, l), a, lane_u, G, un);
 #pragma unroll
             for (int j = 0; j < HU; ++j) {
-                ang.apply(y[j], un, a.interleaved, -1.f);
+                RowVals<T, V, NU> x, y;
+                x.set(xr[j]), y.set(yr[j]);
+                ang.apply(y, un, a.interleaved, -1.f);
                 float ss = 0.f, st = 0.f;
 #pragma unroll
                 for (int i = 0; i < NU; ++i)
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
-                        const float xa = x[j].a[i][e], xb = x[j].b[i][e];
+                        const float xa = x.a[i][e], xb = x.b[i][e];
                         ss = fmaf(xa, xa, fmaf(xb, xb, ss));
-                        st = fmaf(y[j].a[i][e] * wa[i][e], xa, fmaf(y[j].b[i][e] * wb[i][e], xb, st));
+                        st = fmaf(y.a[i][e] * wa[i][e], xa, fmaf(y.b[i][e] * wb[i][e], xb, st));
                     }
-                ss = group_sum<G>(ss), st = group_sum<G>(st);
-                const float r = 1.f / sqrtf(ss / (float)a.E + a.eps);
-                const float k = r * r * (st / (float)a.E);
+                const float r = rsqrtf(fmaf(lanes_sum<G>(ss), inv_e, a.eps));
+                const float k = r * r * (lanes_sum<G>(st) * inv_e);
+                const bool in = h + j < h1;  // (a row of zeros with eps 0 has no r)
 #pragma unroll
                 for (int i = 0; i < NU; ++i)
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
-                        const float xa = x[j].a[i][e], xb = x[j].b[i][e], ya = y[j].a[i][e], yb = y[j].b[i][e];
-                        if (h + j < h1) da[i][e] = fmaf(ya, xa * r, da[i][e]), db[i][e] = fmaf(yb, xb * r, db[i][e]);
-                        x[j].a[i][e] = r * fmaf(ya, wa[i][e], -xa * k);
-                        x[j].b[i][e] = r * fmaf(yb, wb[i][e], -xb * k);
+                        const float xa = x.a[i][e], xb = x.b[i][e], ya = y.a[i][e], yb = y.b[i][e];
+                        if (in) da[i][e] = fmaf(ya, xa * r, da[i][e]), db[i][e] = fmaf(yb, xb * r, db[i][e]);
+                        x.a[i][e] = r * fmaf(ya, wa[i][e], -xa * k);
+                        x.b[i][e] = r * fmaf(yb, wb[i][e], -xb * k);
                     }
-                if (h + j < h1) x[j].store(dst + (int64_t)(h + j) * a.L * a.E, un, a.E);
+                if (in) x.store(dst + (int64_t)(h + j) * a.L * a.E, un, a.E);
             }
         }
     }
@@ -352,30 +334,32 @@ __global__ __launch_bounds__(kThreads) void rotary_norm_bwd_kernel(RotArgs a) {
         }
 }
 
-// dw[d] = the sum over the workgroups' rows: 16 dims per workgroup, 16 threads per dim.
+// dw[d] = the sum over the workgroups' rows: 8 dims per workgroup, 32 threads per dim.
 __global__ __launch_bounds__(256) void rotary_dw_kernel(RotArgs a) {
-    __shared__ float red[16][17];
-    const int which = blockIdx.y, d = blockIdx.x * 16 + (threadIdx.x & 15), p = threadIdx.x >> 4;
+    __shared__ float red[32][9];
+    const int which = blockIdx.y, d = blockIdx.x * 8 + (threadIdx.x & 7), p = threadIdx.x >> 3;
     if (!a.part[which]) return;
     float s = 0.f;
-    if (d < a.E)
-        for (int r = p; r < a.nblk[which]; r += 16) s += a.part[which][(int64_t)r * a.E + d];
-    red[p][threadIdx.x & 15] = s;
+    if (d < a.E) {
+#pragma unroll 8
+        for (int r = p; r < a.nblk[which]; r += 32) s += a.part[which][(int64_t)r * a.E + d];
+    }
+    red[p][threadIdx.x & 7] = s;
     __syncthreads();
     if (p != 0 || d >= a.E) return;
     s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s += red[i][threadIdx.x];
+    for (int i = 0; i < 32; ++i) s += red[i][threadIdx.x];
     if (a.w_bf16) static_cast<__bf16 *>(a.dw[which])[d] = f32_to_bf16(s);
     else static_cast<float *>(a.dw[which])[d] = s;
 }
 
 // 16-byte pieces: whole pieces of pairs and of the dims behind them, rows that start on 16 bytes.
 bool pieces(const RotArgs &a, int V, int size) {
-    if (a.R / 2 % V != 0 || a.E % (2 * V) != 0) return false;
+    if (a.R / 2 % V != 0 || a.E % (2 * V) != 0 || (reinterpret_cast<uintptr_t>(a.freq) & 15) != 0) return false;
     for (const RotRows &t : a.t) {
         if (t.heads == 0) continue;
-        for (const void *p : {t.x, t.g, static_cast<const void *>(t.out)})
+        for (const void *p : {t.x, t.g, t.w, static_cast<const void *>(t.out)})
             if ((reinterpret_cast<uintptr_t>(p) & 15) != 0) return false;
         for (int i = 0; i < 3; ++i)
             if ((t.x && t.xs[i] * size % 16 != 0) || (t.g && t.gs[i] * size % 16 != 0)) return false;
@@ -403,7 +387,7 @@ hipError_t launch_g(const RotArgs &args, bool inverse, bool norm_bwd, hipStream_
     if (a.nblk[0] + a.nblk[1] > 0)
         return_if(launch(rotary_norm_bwd_kernel<T, V, G, NU>, dim3(a.nblk[0] + a.nblk[1]), dim3(kThreads), st, a));
     if (!a.part[0] && !a.part[1]) return hipSuccess;
-    return launch(rotary_dw_kernel, dim3((a.E + 15) / 16, 2), dim3(256), st, a);
+    return launch(rotary_dw_kernel, dim3((a.E + 7) / 8, 2), dim3(256), st, a);
 }
 
 template <typename T>

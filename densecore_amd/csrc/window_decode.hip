@@ -20,26 +20,6 @@ namespace {
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kUnroll = 4;
 constexpr float kShift = 16.f;
 
-template <int CTRL>
-DEVI float dpp_add(float x) {
-    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
-}
-// The sum over LPR neighbouring lanes, in all of them: quads, then quads of 8, halves of 16 (mirrors within
-// the row), 32 and 64.
-template <int LPR>
-DEVI float lanes_sum(float x) {
-    x = dpp_add<0xb1>(x);   // quad_perm [1, 0, 3, 2]
-    x = dpp_add<0x4e>(x);   // quad_perm [2, 3, 0, 1]
-    x = dpp_add<0x141>(x);  // row_half_mirror
-    if (LPR >= 16) x = dpp_add<0x140>(x);  // row_mirror
-    if (LPR >= 32) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-    if (LPR >= 64) x = xor32_add(x);
-    return x;
-}
-
 template <typename T, int CH, bool VEC>
 DEVI void load_piece(const T *row, int d0, int E, float (&x)[CH]) {
     if constexpr (VEC) {
