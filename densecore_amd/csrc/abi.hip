@@ -969,12 +969,14 @@ dc_status window_decode_args(const dc_window_desc *d, dc::WinDecodeArgs *a) {
     a->window = (int)std::min<int64_t>(d->window, INT32_MAX), a->sinks = (int)std::min<int64_t>(d->sinks, INT32_MAX);
     a->scale_log2 = window_scale(d) * 1.4426950408889634f;
     for (int i = 0; i < 3; ++i) a->qs[i] = d->q_stride[i], a->ks[i] = d->k_stride[i], a->vs[i] = d->v_stride[i];
-    a->splits = dc::window_decode_splits(*a, d->dtype == DC_BF16);
     return ok();
 }
 
-size_t window_decode_ws(const dc::WinDecodeArgs &a) {
-    return a.splits > 1 ? round_up((size_t)a.B * a.H * a.splits * (a.E + 2) * sizeof(float)) : 0;
+// The workspace of either plan (which one a call takes depends on its tensors' alignment).
+size_t window_decode_ws(dc::WinDecodeArgs a, bool bf16) {
+    int splits = 1;
+    for (const bool vec : {false, true}) a.vec = vec, splits = std::max(splits, dc::window_decode_splits(a, bf16));
+    return splits > 1 ? round_up((size_t)a.B * a.H * splits * (a.E + 2) * sizeof(float)) : 0;
 }
 
 }  // namespace
@@ -1034,7 +1036,7 @@ dc_status dc_window_bwd(const dc_window_desc *d, const void *grad_out, const voi
 size_t dc_window_decode_workspace_size(const dc_window_desc *d) {
     dc::WinDecodeArgs a;
     if (window_decode_args(d, &a) != DC_OK) return 0;
-    return window_decode_ws(a);
+    return window_decode_ws(a, d->dtype == DC_BF16);
 }
 
 dc_status dc_window_decode(const dc_window_desc *d, const void *q, const void *k, const void *v,
@@ -1050,12 +1052,14 @@ dc_status dc_window_decode(const dc_window_desc *d, const void *q, const void *k
     if (!present(q, nq * a.E) || !present(k, nkv) || !present(v, nkv) || !present(out, nq * a.E) || lse == nullptr ||
         (length_bytes != 0 && lengths == nullptr))
         return fail(DC_INVALID_ARGUMENT, kWindowNull);
-    if (window_decode_ws(a) > 0 && (workspace == nullptr || workspace_bytes < window_decode_ws(a)))
+    const size_t need = window_decode_ws(a, d->dtype == DC_BF16);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(DC_INVALID_ARGUMENT, "window decode workspace is too small");
+    a.vec = window_pieces(d, {q, k, v}, {a.qs, a.ks, a.vs});
+    a.splits = dc::window_decode_splits(a, d->dtype == DC_BF16);
     if ((double)a.B * a.H * a.splits > INT32_MAX / 2) return fail(DC_UNSUPPORTED, "window decode has more than 2^30 pieces");
     a.q = q, a.k = k, a.v = v, a.lengths = lengths, a.length_bytes = length_bytes, a.out = out, a.lse = lse;
     a.part = static_cast<float *>(workspace);
-    a.vec = window_pieces(d, {q, k, v}, {a.qs, a.ks, a.vs});
     return launched(dc::launch_window_decode(a, d->dtype == DC_BF16, static_cast<hipStream_t>(stream)));
 }
 

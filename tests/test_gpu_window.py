@@ -577,3 +577,38 @@ def test_decode_of_large_values(dtype):
         ref = formulas(q, k, v, visible(torch.tensor([S - 1], device=DEV), S, 3500, 4), 0.125, dtype)
         close(F.window_decode(q, k, v, 3500, 4), *ref["out"], dtype, "decode")
         close(F.window_attention(q, k, v, 3500, 4, offset=S - 1), *ref["out"], dtype, "attention")
+
+
+@TYPES
+@pytest.mark.parametrize("heads", [(1, 1), (3, 1), (16, 1), (17, 1), (40, 2), (24, 8)], ids=str)
+def test_decode_heads_that_share_rows(heads, dtype):
+    """Grouped heads of every size, over one piece and several, head dims between the instantiated ones."""
+    from densecore_amd import functional as F
+    H, Hkv = heads
+    gen = torch.Generator().manual_seed(18)
+    for S, E, window, sinks in ((70, 16, 33, 2), (1500, 48, 700, 5), (2600, 120, 2500, 0), (600, 72, 5000, 4)):
+        q, k, v = (torch.randn(2, n, m, E, generator=gen).to(dtype).to(DEV) for n, m in ((H, 1), (Hkv, S), (Hkv, S)))
+        n = torch.tensor([S, S // 2 + 1], device=DEV)
+        open_ = visible(n[:, None] - 1, S, window, sinks)[:, None]
+        ref = formulas(q, k, v, open_, 1 / math.sqrt(E), dtype)
+        close(F.window_decode(q, k, v, window, sinks, lengths=n), *ref["out"], dtype, f"S{S} E{E}")
+
+
+@TYPES
+def test_decode_of_infinite_values(dtype):
+    """An infinite value that is seen makes its dim infinite, and no other; a NaN key makes its sequence NaN."""
+    from densecore_amd import functional as F
+    gen = torch.Generator().manual_seed(19)
+    q, k, v = (torch.randn(3, n, m, 64, generator=gen).to(dtype).to(DEV) for n, m in ((8, 1), (2, 900), (2, 900)))
+    ref = formulas(q, k, v, visible(torch.tensor([899], device=DEV), 900, 600, 4), 0.125, dtype)
+    v2, k2 = v.clone(), k.clone()
+    v2[0, 1, 500, 7] = math.inf
+    v2[1, 0, 899, 63] = -math.inf
+    k2[2, 0, 2] = math.nan
+    out = F.window_decode(q, k2, v2, 600, 4)
+    assert (out[0, 4:, 0, 7] == math.inf).all() and (out[1, :4, 0, 63] == -math.inf).all()
+    assert torch.isnan(out[2, :4]).all()
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[0, 4:, 0, 7] = hit[1, :4, 0, 63] = hit[2, :4] = True
+    value, slack = (t.expand_as(out)[~hit] for t in ref["out"])
+    close(out[~hit], value, slack, dtype, "others")
