@@ -13,6 +13,7 @@ ordered on torch's current stream of the tensors' device.
 """
 import collections
 import contextlib
+import functools
 import math
 
 import torch
@@ -93,7 +94,8 @@ def _ptr(t):
 
 
 def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+    # (As torch.cuda.current_stream(dev).cuda_stream, without the 2 us of a Stream object.)
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 # One workspace per (device, stream), grown on demand and reused: calls on one stream run in
@@ -322,6 +324,24 @@ def _unit_rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+_S3 = _lib.ctypes.c_int64 * 3
+
+
+def _strides(t):
+    return _S3() if t is None else _S3(*t[:3])
+
+
+# A descriptor depends on sizes, strides and options alone, and is never written to once made.
+@functools.lru_cache(maxsize=256)
+def _rotary_struct(*fields):
+    return _lib.RotaryDesc(*fields[:17], *(_strides(t) for t in fields[17:]))
+
+
+@functools.lru_cache(maxsize=256)
+def _window_struct(*fields):
+    return _lib.WindowDesc(*fields[:12], *(_strides(t) for t in fields[12:]))
+
+
 def _rotary_desc(q, k, inv_freq, positions, offset, interleaved, magnitude, eps, weights, grads=(None, None)):
     """Checks the arguments of the rotation; returns its descriptor (``dc_rotary_desc``)."""
     if q.dim() != 4 or (k is not None and k.dim() != 4):
@@ -341,18 +361,16 @@ def _rotary_desc(q, k, inv_freq, positions, offset, interleaved, magnitude, eps,
         raise ValueError("rotary inv_freq must be a float64 vector on the tensors' device")
     if 2 * inv_freq.shape[0] > E:
         raise ValueError("rotary inv_freq turns more dims than the head has")
-    wtype = _DTYPES[q.dtype]
+    wdtype = None
     for w in weights or ():
         if w is None:
             continue
         if tuple(w.shape) != (E,) or w.dtype not in _DTYPES or w.device != dev:
             raise ValueError("norm weights must be float32 or bfloat16 vectors of head_dim values on the "
                              "tensors' device")
-    given = {w.dtype for w in weights or () if w is not None}
-    if len(given) > 1:
-        raise ValueError("norm weights must share one dtype")
-    for dtype in given:
-        wtype = _DTYPES[dtype]
+        if wdtype not in (None, w.dtype):
+            raise ValueError("norm weights must share one dtype")
+        wdtype = w.dtype
     pos_bytes, ps = 0, (0, 0)
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64) or positions.device != dev:
@@ -363,13 +381,9 @@ def _rotary_desc(q, k, inv_freq, positions, offset, interleaved, magnitude, eps,
             raise ValueError("rotary takes positions or an offset, not both")
         pos_bytes = positions.element_size()
         ps = (positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0, positions.stride(-1))
-    S3 = _lib.ctypes.c_int64 * 3
-
-    def strides(t):
-        return S3(*t.stride()[:3]) if t is not None else S3()
-    return _lib.RotaryDesc(B, H, 0 if k is None else k.shape[1], L, E, 2 * inv_freq.shape[0], _DTYPES[q.dtype],
-                           wtype, int(bool(interleaved)), int(weights is not None), pos_bytes, 0, int(offset), *ps,
-                           float(magnitude), float(eps), strides(q), strides(k), strides(grads[0]), strides(grads[1]))
+    return _rotary_struct(B, H, 0 if k is None else k.shape[1], L, E, 2 * inv_freq.shape[0], _DTYPES[q.dtype],
+                          _DTYPES[wdtype or q.dtype], interleaved, weights is not None, pos_bytes, 0, offset, *ps,
+                          magnitude, eps, *(None if t is None else t.stride() for t in (q, k, *grads)))
 
 
 def _rotary(q, k, inv_freq, positions=None, offset=0, interleaved=False, magnitude=1.0, weights=None, eps=0.0):
@@ -431,10 +445,9 @@ def _window_desc(q, k, v, window, sinks, offset, scale, grad_out=None):
     for t in (k, v, grad_out):
         if t is not None and (t.device != q.device or t.dtype != q.dtype):
             raise ValueError("window attention tensors must share one device and dtype")
-    S3 = _lib.ctypes.c_int64 * 3
-    return _lib.WindowDesc(B, H, Hkv, L, S, E, offset, min(window, 2 ** 31), min(sinks, 2 ** 31), _DTYPES[q.dtype],
-                           int(scale is not None), 0.0 if scale is None else scale,
-                           *(S3(*t.stride()[:3]) if t is not None else S3() for t in (q, k, v, grad_out)))
+    return _window_struct(B, H, Hkv, L, S, E, offset, min(window, 2 ** 31), min(sinks, 2 ** 31), _DTYPES[q.dtype],
+                          scale is not None, 0.0 if scale is None else scale,
+                          *(None if t is None else t.stride() for t in (q, k, v, grad_out)))
 
 
 def _window_attention(q, k, v, window, sinks=0, offset=0, scale=None, with_rest=False):

@@ -184,8 +184,7 @@ __global__ __launch_bounds__(kThreads) void window_decode_kernel(WinDecodeArgs a
 // rows (S^T = K Q^T, keys x heads) nor the transposed ones (O^T = V^T P^T) meet in a bank.  P enters as two bf16
 // terms, carried to 2^-17; in v_mfma_f32_16x16x32_bf16's layouts a lane holds a head's scores of keys
 // 4 (l / 16) + 0..3 of both 16-key halves, which is what the second product takes.
-typedef float f32x4v __attribute__((ext_vector_type(4)));
-DEVI f32x4v mfma16(bf16x8 a, bf16x8 b, f32x4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+DEVI f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 constexpr int kTile = 32, kHeads = 16;
 
 template <int D>
@@ -252,9 +251,9 @@ __global__ __launch_bounds__(kThreads) void window_decode_mfma_kernel(WinDecodeA
     bf16x8 qf[KST];
 #pragma unroll
     for (int st = 0; st < KST; ++st) qf[st] = Ops<__bf16>::load<true>(qb + lh * a.qs[1], 32 * st + 8 * g, a.E, lh < nh);
-    f32x4v acc[NDT];
+    f32x4 acc[NDT];
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) acc[dt] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    for (int dt = 0; dt < NDT; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_part = 0.f;
     // What a lane reads of the tile: row lh's chunks of both halves, and for the transposed reads
     // row 4 g + lh / 4, dims 4 (lh % 4) + 0..3 of 16.
@@ -267,7 +266,7 @@ __global__ __launch_bounds__(kThreads) void window_decode_mfma_kernel(WinDecodeA
         float mx = -INFINITY;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            f32x4v c = {0.f, 0.f, 0.f, 0.f};
+            f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int st = 0; st < KST; ++st)
                 c = mfma16(__builtin_bit_cast(bf16x8, kt[x].x[RowTile<D>::slot(16 * h + lh, 4 * st + g)]), qf[st], c);

@@ -301,22 +301,43 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
 }
 
 // Joins the pieces of each row, 16 lanes per row: lse = log sum exp(lse_i), out = sum exp(lse_i - lse) o_i.
-template <typename T>
+// The lanes form the pieces' weights once (LDS), then each sums 4 dims at a time.
+constexpr int kMaxSplits = 128;
+template <typename T, bool VEC4>
 __global__ __launch_bounds__(256) void window_merge_kernel(WinArgs a) {
+    __shared__ float weight[16][kMaxSplits + 1];
     const int64_t nrows = (int64_t)a.B * a.H * a.L, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (row >= nrows) return;
-    const int part = threadIdx.x & 15;
-    float top = -INFINITY, sum = 0.f;
-    for (int i = 0; i < a.splits; ++i) top = fmaxf(top, a.part_lse[i * nrows + row]);
+    if (row >= nrows) return;  // (whole groups of lanes; a row's weights are its own lanes' alone)
+    const int part = threadIdx.x & 15, r = threadIdx.x >> 4;
+    float top = -INFINITY;
+    for (int i = part; i < a.splits; i += 16) top = fmaxf(top, weight[r][i] = a.part_lse[i * nrows + row]);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     const float base = top == -INFINITY ? 0.f : top;
-    for (int i = 0; i < a.splits; ++i) sum += exp2_fast((a.part_lse[i * nrows + row] - base) * kLog2e);
+    float sum = 0.f;
+    for (int i = part; i < a.splits; i += 16) sum += weight[r][i] = exp2_fast((weight[r][i] - base) * kLog2e);
+    sum = lanes_sum<16>(sum);
     const bool empty = sum == 0.f;
     const float inv = empty ? 0.f : 1.f / sum;
-    for (int d = part; d < a.E; d += 16) {
-        float o = 0.f;
-        for (int i = 0; i < a.splits; ++i)
-            o = fmaf(exp2_fast((a.part_lse[i * nrows + row] - base) * kLog2e) * inv, a.part[(i * nrows + row) * a.E + d], o);
-        put<T>(a, row * a.E + d, o);
+    wait_lds();
+    for (int d = 4 * part; d < a.E; d += 64) {
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int i = 0; i < a.splits; ++i) {
+            const float *p = a.part + (i * nrows + row) * a.E + d, w = weight[r][i] * inv;
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (VEC4) {
+                x = *reinterpret_cast<const f32x4 *>(p);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = d + e < a.E ? p[e] : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[e], o[e]);
+        }
+        store4<T, false>(static_cast<T *>(a.out) + row * a.E, d, a.E, o[0], o[1], o[2], o[3]);
+        if (sizeof(T) == 2 && a.rest)
+            store4<T, false>(static_cast<T *>(a.rest) + row * a.E, d, a.E, rest_of(o[0]), rest_of(o[1]), rest_of(o[2]), rest_of(o[3]));
     }
     if (part == 0) a.lse[row] = empty ? 0.f : base + log2_fast(sum) * kLn2;
 }
@@ -329,15 +350,15 @@ int64_t blocks_of(const WinArgs &a, bool pack) {
     return (rows + kM - 1) / kM * a.B * (a.H / (pack ? a.repeat : 1));
 }
 
-// Pieces of each tile's keys: where the tiles fill at most half of the CUs, as many as fill them, of at
-// least 256 keys.
+// Pieces of each tile's keys: where the tiles fill at most half of the CUs, as many as give each CU two
+// workgroups, of at least 256 keys.
 int plan_splits(const WinArgs &a, bool bf16) {
     const int64_t blocks = blocks_of(a, packs(a)), cus = device_cus();
     if (blocks == 0 || cus <= 0 || 2 * blocks > cus) return 1;
     const int BN = bf16 ? kKeys<__bf16> : kKeys<float>;
     const int64_t span = std::min<int64_t>(a.S, (int64_t)a.window + a.sinks + std::min(a.L, kM));
     const int64_t most = std::max<int64_t>(1, span / std::max(256, BN));
-    return (int)std::min(most, cus / blocks);
+    return (int)std::min<int64_t>({most, 2 * cus / blocks, kMaxSplits});
 }
 
 template <typename T, int D, bool VEC>
@@ -345,7 +366,9 @@ hipError_t launch_v(const WinArgs &a, hipStream_t st) {
     return_if(launch(window_fwd_kernel<T, D, VEC>, dim3((unsigned)(blocks_of(a, a.pack) * a.splits)), dim3(kThreads), st, a));
     if (a.splits == 1) return hipSuccess;
     const int64_t nrows = (int64_t)a.B * a.H * a.L;
-    return launch(window_merge_kernel<T>, dim3((unsigned)((nrows + 15) / 16)), dim3(256), st, a);
+    const dim3 grid((unsigned)((nrows + 15) / 16)), block(256);
+    return a.E % 4 == 0 ? launch(window_merge_kernel<T, true>, grid, block, st, a)
+                        : launch(window_merge_kernel<T, false>, grid, block, st, a);
 }
 template <typename T, int D>
 hipError_t launch_d(const WinArgs &a, hipStream_t st) {
