@@ -43,8 +43,9 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nqt = (a.L + kM - 1) / kM;
     const int w = logical_block();
-    const int qt = nqt - 1 - w % nqt, bh = w / nqt;
-    const int b = bh / a.H, h = bh % a.H, hk = h / a.repeat;
+    // (The heads of a kv head side by side, as in the forward.)
+    const int qt = nqt - 1 - w / a.repeat % nqt, kvh = w / a.repeat / nqt;
+    const int b = kvh / a.Hkv, hk = kvh % a.Hkv, h = hk * a.repeat + w % a.repeat, bh = b * a.H + h;
     const int r0 = qt * kM, wr0 = r0 + 32 * wave, r = wr0 + lr;
     const bool in = r < a.L;
     const int l = in ? r : a.L - 1, p = in ? a.offset + l : -1;

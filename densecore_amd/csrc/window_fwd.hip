@@ -154,13 +154,16 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) v
 
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int G = a.pack ? a.repeat : 1, rows = G * a.L, groups = a.H / G;
+    const int G = a.pack ? a.repeat : 1, rows = G * a.L;
     const int nqt = (rows + kM - 1) / kM;
     int w = logical_block();
     const int piece = w % a.splits;
     w /= a.splits;
-    const int qt = nqt - 1 - w % nqt, grp = w / nqt;
-    const int b = grp / groups, h0 = grp % groups * G, hk = h0 / a.repeat;
+    // The heads (groups of heads) of a kv head side by side, then its row tiles, longest first: the workgroups
+    // an XCD runs at once read few keys.
+    const int share = a.repeat / G;
+    const int qt = nqt - 1 - w / share % nqt, kvh = w / share / nqt;
+    const int b = kvh / a.Hkv, hk = kvh % a.Hkv, h0 = hk * a.repeat + w % share * G;
     const int r0 = qt * kM, wr0 = r0 + 32 * wave, r = wr0 + lr;
     const bool in = r < rows;
     const RowAt at = row_at(a, in ? r : rows - 1);
