@@ -108,6 +108,8 @@ __host__ __device__ inline Band band_of(int p0, int p1, int S, int window, int s
     return b;
 }
 
+#define lds __attribute__((address_space(3)))  // pointers into LDS
+
 // Operands of one type.
 template <typename T>
 struct Ops;
@@ -216,17 +218,30 @@ struct Stage<__bf16, R, D, THREADS, true> {
         constexpr int W = THREADS / 64, RB = R / 64 ? R / 64 : 1, NT = CMTile<R, D>::C * RB, count = (NT + W - 1) / W;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
         const uint32_t loff = (uint32_t)lane * (uint32_t)(ld * 2);
+        // Transfer x moves chunk x / RB of rows 64 (x % RB) + lane.
+        if (R >= 64 && NT % (2 * W) == 0 && rows >= R && E == D) {
+            // Whole tiles in straight lines, two transfers a statement: their tests and address arithmetic are a
+            // wave's own time (forward B2 H32/8 L8192 E128 W1024 459 -> 444 us, B4 H32 L4096 E64 279 -> 262).
+            const uint32_t to = (uint32_t)(uintptr_t)(const lds u32x4 *)t.p;
+            const uint64_t from = sgpr_addr(src), block = sgpr_addr(src + 64 * ld) - from;
+#pragma unroll
+            for (int j = 0; j < count; j += 2) {
+                const int x = wave + W * j, y = x + W;
+                const uint64_t gx = from + 16 * (x / RB) + x % RB * block, gy = from + 16 * (y / RB) + y % RB * block;
+                const uint32_t lx = to + 16 * (x / RB * CMTile<R, D>::P + 64 * (x % RB));
+                const uint32_t ly = to + 16 * (y / RB * CMTile<R, D>::P + 64 * (y % RB));
+                lds_dma16_pair(gx, loff, lx, gy, loff, ly);
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < count; ++j) {
             const int inst = wave + W * j, c = inst / RB, rb = inst % RB;
             if (inst >= NT || 8 * c >= E) continue;  // wave-uniform
             u32x4 *d = t.p + c * CMTile<R, D>::P + 64 * rb;
-            const __bf16 *s = src + (int64_t)(64 * rb) * ld + 8 * c;
             const int row = 64 * rb + lane;
-            if (R >= 64 && rows >= R) {
-                lds_dma16_off(s, loff, d);
-            } else if (row < R) {
-                if (row < rows) lds_dma16_off(s, loff, d);
+            if (row < R) {
+                if (row < rows) lds_dma16_off(src + (int64_t)(64 * rb) * ld + 8 * c, loff, d);
                 else d[lane] = u32x4{0u, 0u, 0u, 0u};
             }
         }

@@ -18,7 +18,7 @@ namespace {
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kM = 32 * kWaves;
 template <typename T>
 constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // dQ: keys per tile
-// Two waves per SIMD, but for float32 at D = 128 (three parts of two operands and the sums take 350 registers).
+// Two waves per SIMD or more, but for float32 at D = 128 (three parts of two operands and the sums take 350 registers).
 template <typename T, int D>
 constexpr int kWavesPerSimd = sizeof(T) == 2 || D <= 64 ? 2 : 1;
 // dK / dV: waves w and w + 4 own the same 32 keys and halve each step's queries (one wave per SIMD: no halves).
@@ -33,7 +33,7 @@ constexpr bool kVLds = D >= 64 && (sizeof(T) == 2 ? D == 128 : D == 64);
 
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(kThreads)
-__attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) void window_dq_kernel(WinArgs a) {
+__attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dq_kernel(WinArgs a) {
     typedef Ops<T> O;
     constexpr int BN = kKeys<T>, NT = BN / 32, KSTEP = D / 16, NDT = D / 32;
     typedef Stage<T, BN, D, kThreads, VEC> St;
@@ -220,7 +220,7 @@ DEVI Pieces pieces_of(const WinArgs &a, int nkt, int bhk, int kt) {
 
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__((kThreads * kHalves<T, D>))
-__attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) void window_dkdv_kernel(WinArgs a) {
+__attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dkdv_kernel(WinArgs a) {
     typedef Ops<T> O;
     constexpr int HALVES = kHalves<T, D>, QM = 32 * HALVES, THREADS = kThreads * HALVES, KSTEP = D / 16, NDT = D / 32;
     constexpr bool KLDS = kKLds<T, D>, VLDS = kVLds<T, D>;

@@ -22,6 +22,8 @@ template <typename T>
 constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // keys per tile
 template <typename T, int D>
 constexpr int kWavesPerSimd = sizeof(T) == 2 || D <= 64 ? 2 : 1;  // LDS: 110 KB of float32 tiles at D = 128
+// ... as the least.  bf16 at D = 64 runs four, whose products cover each other's softmax (B4 H32 L4096 W1024
+// 262 -> 227 us against two), at D = 32 too (225 -> 165); at D = 128 two workgroups' tiles fill the LDS.
 
 // Row r of a group of `pack`ed heads (or of one head) as (head within the group, query).
 struct RowAt {
@@ -146,7 +148,7 @@ DEVI void write_rows(const WinArgs &a, const f32x16 (&acc)[D / 32], float m_run,
 
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(kThreads)
-__attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>, kWavesPerSimd<T, D>))) void window_fwd_kernel(WinArgs a) {
+__attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_fwd_kernel(WinArgs a) {
     typedef Ops<T> O;
     constexpr int BN = kKeys<T>, NT = BN / 32, KSTEP = D / 16, NDT = D / 32;
     typedef Stage<T, BN, D, kThreads, VEC> St;
