@@ -324,6 +324,12 @@ def _unit_rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _scratch(nbytes, dev):
+    """A workspace of one call's own (None: the call takes none).  Two host threads that call on one stream
+    have their launches interleaved, so calls of several kernels do not share a stream's workspace."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
 _S3 = _lib.ctypes.c_int64 * 3
 
 
@@ -382,7 +388,8 @@ def _rotary_desc(q, k, inv_freq, positions, offset, interleaved, magnitude, eps,
         pos_bytes = positions.element_size()
         ps = (positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0, positions.stride(-1))
     return _rotary_struct(B, H, 0 if k is None else k.shape[1], L, E, 2 * inv_freq.shape[0], _DTYPES[q.dtype],
-                          _DTYPES[wdtype or q.dtype], interleaved, weights is not None, pos_bytes, 0, offset, *ps,
+                          _DTYPES[wdtype or q.dtype], interleaved, weights is not None, pos_bytes, 0,
+                          max(-2 ** 62, min(offset, 2 ** 62)), *ps,
                           magnitude, eps, *(None if t is None else t.stride() for t in (q, k, *grads)))
 
 
@@ -422,7 +429,7 @@ def _rotary_backward(grad_q, grad_k, q, k, inv_freq, positions=None, offset=0, i
     x = (q, k) if weights is not None else (None, None)
     L_ = _lib.lib()
     with _on(dev):
-        ws = _workspace(L_.dc_rotary_bwd_workspace_size(d), dev) if dwq is not None or dwk is not None else None
+        ws = _scratch(L_.dc_rotary_bwd_workspace_size(d), dev) if dwq is not None or dwk is not None else None
         _lib.check(L_.dc_rotary_bwd(d, _ptr(grad_q), _ptr(grad_k), _ptr(x[0]), _ptr(x[1]), _ptr(wq), _ptr(wk),
                                     _ptr(inv_freq), _ptr(positions), _ptr(dq), _ptr(dk), _ptr(dwq), _ptr(dwk),
                                     _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev)))
@@ -445,8 +452,8 @@ def _window_desc(q, k, v, window, sinks, offset, scale, grad_out=None):
     for t in (k, v, grad_out):
         if t is not None and (t.device != q.device or t.dtype != q.dtype):
             raise ValueError("window attention tensors must share one device and dtype")
-    return _window_struct(B, H, Hkv, L, S, E, offset, min(window, 2 ** 31), min(sinks, 2 ** 31), _DTYPES[q.dtype],
-                          scale is not None, 0.0 if scale is None else scale,
+    return _window_struct(B, H, Hkv, L, S, E, min(offset, 2 ** 31), min(window, 2 ** 31), min(sinks, 2 ** 31),
+                          _DTYPES[q.dtype], scale is not None, 0.0 if scale is None else scale,
                           *(None if t is None else t.stride() for t in (q, k, v, grad_out)))
 
 
@@ -460,8 +467,7 @@ def _window_attention(q, k, v, window, sinks=0, offset=0, scale=None, with_rest=
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
     rest = torch.empty_like(out) if with_rest and q.dtype == torch.bfloat16 else None
     with _on(dev):
-        nbytes = L_.dc_window_fwd_workspace_size(d)
-        ws = _workspace(nbytes, dev) if nbytes else None
+        ws = _scratch(L_.dc_window_fwd_workspace_size(d), dev)
         _lib.check(L_.dc_window_fwd(d, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(lse), _ptr(ws),
                                     0 if ws is None else ws.numel(), _stream(dev)))
     return (out, lse, rest) if with_rest else (out, lse)
@@ -481,9 +487,9 @@ def _window_attention_backward(grad_out, q, k, v, out, lse, rest, window, sinks=
     out, lse, rest = out.contiguous(), lse.contiguous(), None if rest is None else rest.contiguous()
     dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v))
     with _on(dev):
-        ws = _workspace(L_.dc_window_bwd_workspace_size(d), dev)
+        ws = _scratch(L_.dc_window_bwd_workspace_size(d), dev)
         _lib.check(L_.dc_window_bwd(d, _ptr(grad_out), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(lse),
-                                    _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream(dev)))
+                                    _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev)))
     return dq, dk, dv
 
 
@@ -500,8 +506,7 @@ def _window_decode(q, k, v, window, sinks=0, lengths=None, scale=None):
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
     with _on(dev):
-        nbytes = L_.dc_window_decode_workspace_size(d)
-        ws = _workspace(nbytes, dev) if nbytes else None
+        ws = _scratch(L_.dc_window_decode_workspace_size(d), dev)
         _lib.check(L_.dc_window_decode(d, _ptr(q), _ptr(k), _ptr(v), _ptr(lengths),
                                        0 if lengths is None else lengths.element_size(), _ptr(out), _ptr(lse),
                                        _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev)))

@@ -800,6 +800,8 @@ dc_status check_rotary(const dc_rotary_desc *d, const double *inv_freq, const vo
     if (d->pos_bytes != 0 && d->pos_bytes != 4 && d->pos_bytes != 8)
         return fail(DC_INVALID_ARGUMENT, "rotary positions must be int32 or int64");
     if (d->reserved != 0) return fail(DC_INVALID_ARGUMENT, "rotary descriptor's reserved field must be 0");
+    if (d->offset > ((int64_t)1 << 53) || d->offset < -((int64_t)1 << 53))
+        return fail(DC_UNSUPPORTED, "rotary offset exceeds 2^53");  // (positions are formed in float64)
     for (int i = 0; i < 3; ++i)
         if (d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->grad_q_stride[i] < 0 || d->grad_k_stride[i] < 0)
             return fail(DC_INVALID_ARGUMENT, "rotary strides must be non-negative");
@@ -903,7 +905,7 @@ dc_status check_window(const dc_window_desc *d, int max_head_dim) {
     if (d->window < 1) return fail(DC_INVALID_ARGUMENT, "window attention window must be at least 1");
     if (d->sinks < 0) return fail(DC_INVALID_ARGUMENT, "window attention sinks must not be negative");
     if (d->offset < 0) return fail(DC_INVALID_ARGUMENT, "window attention offset must not be negative");
-    if (d->has_scale && !std::isfinite((float)d->scale))
+    if (d->has_scale && !std::isfinite((float)d->scale * 1.4426950408889634f))  // (as the kernels take it)
         return fail(DC_INVALID_ARGUMENT, "window attention scale must be finite");
     for (int i = 0; i < 3; ++i)
         if (d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0 || d->grad_out_stride[i] < 0)
@@ -935,7 +937,8 @@ dc_status window_args(const dc_window_desc *d, dc::WinArgs *a) {
     if (st != DC_OK) return st;
     const int64_t rows = (d->q_len + 31) / 32 + 1, keys = (d->kv_len + 31) / 32 + 1;
     if (d->batch * d->heads > INT32_MAX / 2 || (double)d->batch * d->heads * rows > INT32_MAX / 2 ||
-        (double)d->batch * d->kv_heads * keys > INT32_MAX / 2)
+        (double)d->batch * d->kv_heads * keys > INT32_MAX / 2 ||
+        (double)(d->heads / d->kv_heads) * d->q_len * (d->q_len <= 64) > INT32_MAX / 2)  // rows of packed heads
         return fail(DC_UNSUPPORTED, "window attention has more than 2^30 tiles");
     *a = dc::WinArgs{};
     a->B = (int)d->batch, a->H = (int)d->heads, a->Hkv = (int)d->kv_heads;

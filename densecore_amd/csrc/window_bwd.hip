@@ -495,8 +495,11 @@ void plan_pieces(WinArgs &a, bool bf16) {
     a.sink_tiles = (int)std::min<int64_t>(nkt, ((int64_t)a.sinks + kM - 1) / kM);
     a.sink_pieces = a.tile_pieces = 1;
     if (nkt == 0 || a.L == 0 || a.B * a.Hkv == 0) return;
-    int64_t most = 0;  // steps of the longest tile without sinks
-    for (int kt = a.sink_tiles; kt < nkt; ++kt) most = std::max(most, tile_steps(a, kt * kM, QM));
+    // Steps of the longest tile without sinks: its queries grow in number up to the tile of the first query's
+    // position, and do not behind the next.
+    int64_t most = 0;
+    for (int kt = a.offset / kM; kt <= a.offset / kM + 1 && nkt > a.sink_tiles; ++kt)
+        most = std::max(most, tile_steps(a, std::clamp(kt, a.sink_tiles, nkt - 1) * kM, QM));
     const int64_t heads = (int64_t)a.B * a.Hkv, cus = std::max(device_cus(), 1), rest = nkt - a.sink_tiles;
     if (rest > 0 && most > 0)
         a.tile_pieces = (int)std::max<int64_t>(1, std::min<int64_t>(most / 4, cus / (heads * rest)));

@@ -421,6 +421,11 @@ def _turn_args(offset, interleaved, magnitude):
     return int(offset), interleaved, float(magnitude)
 
 
+def _refuse_frequency_gradient(inv_freq):
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("rotary inv_freq has no gradient")
+
+
 def _check_tensors(what, **tensors):
     for name, t in tensors.items():
         if not isinstance(t, torch.Tensor):
@@ -439,6 +444,7 @@ def rotary_embedding(query, key, inv_freq, positions=None, offset=0, interleaved
     _check_tensors("rotary", query=query, inv_freq=inv_freq, **({} if key is None else {"key": key}),
                    **({} if positions is None else {"positions": positions}))
     args = _turn_args(offset, interleaved, magnitude)
+    _refuse_frequency_gradient(inv_freq)
     if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
         q, k = _Rotary.apply(query, key, None, None, False, inv_freq, positions, args, 0.0)
     else:
@@ -458,6 +464,7 @@ def qk_norm_rotary(query, key, query_weight, key_weight, inv_freq, positions=Non
                    **({} if positions is None else {"positions": positions}),
                    **{n: w for n, w in (("query_weight", query_weight), ("key_weight", key_weight)) if w is not None})
     args = _turn_args(offset, interleaved, magnitude)
+    _refuse_frequency_gradient(inv_freq)
     if isinstance(eps, bool) or not isinstance(eps, numbers.Real):
         raise TypeError("norm eps must be real")
     if not eps >= 0:

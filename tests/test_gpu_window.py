@@ -612,3 +612,63 @@ def test_decode_of_infinite_values(dtype):
     hit[0, 4:, 0, 7] = hit[1, :4, 0, 63] = hit[2, :4] = True
     value, slack = (t.expand_as(out)[~hit] for t in ref["out"])
     close(out[~hit], value, slack, dtype, "others")
+
+
+@pytest.mark.parametrize("offset", [2 ** 30, 2 ** 31 + 1, 2 ** 64, 2 ** 64 + 5])
+def test_offsets_out_of_range(offset):
+    from densecore_amd import functional as F
+    x = torch.zeros(1, 2, 3, 8, device=DEV)
+    with pytest.raises(NotImplementedError, match="offset"):
+        F.window_attention(x, x, x, 4, 0, offset)
+    f = torch.zeros(4, dtype=torch.float64, device=DEV)
+    if offset >= 2 ** 53:
+        for o in (offset, -offset):
+            with pytest.raises(NotImplementedError, match="offset"):
+                F.rotary_embedding(x, x, f, offset=o)
+
+
+def test_host_threads_on_one_stream():
+    """Calls of several kernels from host threads whose launches interleave on one stream."""
+    import threading
+    from densecore_amd import functional as F
+    gen = torch.Generator().manual_seed(31)
+    xs = [[torch.randn(1, n, 2000, 64, generator=gen).to(DEV) for n in (4, 2, 2, 4)] for _ in range(4)]
+
+    def work(q, k, v, g):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        few = F.window_attention(q[:, :, -3:], k, v, 1900, 4, offset=1997)
+        one = F.window_decode(q[:, :, -1:], k, v, 1900, 4)
+        return (few, one, *torch.autograd.grad(F.window_attention(*leaves, 100, 4), leaves, g))
+    ref = [work(*x) for x in xs]
+    torch.cuda.synchronize()
+    got = [[] for _ in xs]
+
+    def run(i):
+        for _ in range(10):
+            got[i].append(work(*xs[i]))
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for a, runs in zip(ref, got):
+        assert len(runs) == 10
+        assert all(torch.equal(s, t) for b in runs for s, t in zip(a, b))
+
+
+@pytest.mark.parametrize("sizes", [(1, 700, 700, 0, 0), (300, 2000, 200, 1700, 4), (2000, 300, 64, 0, 0),
+                                   (500, 1500, 128, 250, 200), (64, 1111, 3000, 900, 0)], ids=str)
+def test_gradient_pieces(sizes):
+    """The longest key tile without sinks, which sets the pieces, wherever it lies."""
+    from densecore_amd import functional as F
+    L, S, window, offset, sinks = sizes
+    gen = torch.Generator().manual_seed(L + S)
+    q, k, v, g = (torch.randn(1, h, n, 32, generator=gen).to(DEV) for h, n in ((2, L), (1, S), (1, S), (2, L)))
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    y = F.window_attention(*leaves, window, sinks, offset)
+    dq, dk, dv = torch.autograd.grad(y, leaves, g)
+    open_ = visible(torch.arange(offset, offset + L, device=DEV), S, window, sinks)
+    ref = formulas(q, k, v, open_, 32 ** -0.5, torch.float32, g)
+    for name, x in (("out", y), ("dq", dq), ("dk", dk), ("dv", dv)):
+        close(x, *ref[name], torch.float32, name)

@@ -129,3 +129,20 @@ def test_c_entries_refuse_pointers():
     assert L.dc_rotary_bwd(n, P, P, None, P, P, P, P, P, P, P, P, P, P, size, None) == bad
     # No tokens: nothing to do.
     assert L.dc_rotary_fwd(_desc(batch=0), None, None, None, None, None, None, None, None, None) == _lib.DC_OK
+
+
+@pytest.mark.parametrize("offset", [2 ** 53 + 1, -2 ** 53 - 1, 2 ** 62])
+def test_offsets_that_float64_does_not_hold_are_refused(offset):
+    L, d = _lib.lib(), _desc(offset=offset)
+    assert L.dc_rotary_fwd(d, P, P, None, None, P, P, P, P, None) == _lib.DC_UNSUPPORTED
+    assert L.dc_rotary_bwd(d, P, P, P, P, None, None, P, P, P, P, None, None, None, 0, None) == _lib.DC_UNSUPPORTED
+
+
+def test_frequencies_have_no_gradient():
+    x, f = torch.zeros(1, 2, 3, 4), torch.zeros(2, dtype=torch.float64, requires_grad=True)
+    with pytest.raises(NotImplementedError, match="gradient"):
+        functional.rotary_embedding(x, x, f)
+    with pytest.raises(NotImplementedError, match="gradient"):
+        functional.qk_norm_rotary(x, x, None, None, f)
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+        functional.rotary_embedding(x, x, f)

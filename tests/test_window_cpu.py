@@ -84,3 +84,12 @@ def test_c_entries_refuse_pointers_and_workspaces():
     # Nothing to compute: no pointer is looked at.
     assert L.dc_window_fwd(_desc(batch=0), *[None] * 7, 0, None) == _lib.DC_OK
     assert L.dc_window_decode(_desc(batch=0), None, None, None, None, 0, None, None, None, 0, None) == _lib.DC_OK
+
+
+def test_numbers_past_the_kernels_range_are_refused():
+    """A scale that is finite until it is taken in base 2, packed rows past 2^30."""
+    L = _lib.lib()
+    assert L.dc_window_fwd(_desc(has_scale=1, scale=3e38), P, P, P, P, None, P, None, 0, None) == _lib.DC_INVALID_ARGUMENT
+    many = _desc(heads=2 ** 28, kv_heads=1, q_len=32, head_dim=1)
+    assert L.dc_window_fwd(many, P, P, P, P, None, P, None, 0, None) == _lib.DC_UNSUPPORTED
+    assert L.dc_window_bwd(many, *[P] * 11, 1 << 40, None) == _lib.DC_UNSUPPORTED
