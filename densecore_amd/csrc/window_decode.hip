@@ -383,6 +383,8 @@ __global__ __launch_bounds__(64) void window_decode_merge_kernel(WinDecodeArgs a
     if (lane == 0) a.lse[row] = t == 0.f ? 0.f : (ref + kShift + log2_fast(t)) * kLn2;
 }
 
+// The heads that share a row's registers: float32 B8, 8 kv heads, 4096 keys with 8 heads each 80 us, and 171 with a
+// workgroup per head; 4 heads 58 and 86.
 int heads_per_block(int repeat) { return repeat >= 5 ? 8 : repeat >= 3 ? 4 : repeat; }
 
 bool on_mfma(const WinDecodeArgs &a, bool bf16) { return bf16 && a.vec && a.E <= 128; }
@@ -419,14 +421,16 @@ hipError_t launch_v(const WinDecodeArgs &a, hipStream_t st) {
 
 }  // namespace
 
-// Pieces of a sequence's keys: as many as give every CU four workgroups (two of the MFMA kernel's, whose
-// buffers fill a CU's LDS), of at least 128 keys.
+// Pieces of a sequence's keys, of at least 128: as many as give every CU one workgroup of the MFMA kernel, whose
+// buffers fill its LDS (with two of them in turn B16 H32/8 E128 over the last 4096 keys takes 60 us and not 57, B2 with
+// 8192 keys 27 and not 21), and two of the other (float32 B8 H32/8, 4096 keys: 64 us with one, 51 with two, 58
+// with four).
 int window_decode_splits(const WinDecodeArgs &a, bool bf16) {
     const int per = on_mfma(a, bf16) ? kHeads : heads_per_block(a.repeat);
     const int64_t blocks = (int64_t)a.B * a.Hkv * ((a.repeat + per - 1) / per);
     const int64_t span = std::min<int64_t>(a.S, (int64_t)a.window + a.sinks), cus = std::max(device_cus(), 1);
     if (blocks == 0) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(span / 128, (on_mfma(a, bf16) ? 2 : 4) * cus / blocks));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(span / 128, (on_mfma(a, bf16) ? 1 : 2) * cus / blocks));
 }
 
 hipError_t launch_window_decode(const WinDecodeArgs &a, bool bf16, hipStream_t st) {

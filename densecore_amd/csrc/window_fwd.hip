@@ -347,7 +347,8 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinArgs a) {
     if (part == 0) a.lse[row] = empty ? 0.f : base + log2_fast(sum) * kLn2;
 }
 
-// Heads that share a kv head share tiles where a head's queries fill less than half of one.
+// Heads that share a kv head share tiles where a head's queries fill at most half of one: B64 H32/8, 16 rows each over
+// 1124 keys bf16 66 us, 171 apart; 48 rows, B16, 44 and 59; with 100 rows it no longer matters (68, 68).
 bool packs(const WinArgs &a) { return a.repeat > 1 && a.L <= kM / 2; }
 
 int64_t blocks_of(const WinArgs &a, bool pack) {
@@ -355,15 +356,18 @@ int64_t blocks_of(const WinArgs &a, bool pack) {
     return (rows + kM - 1) / kM * a.B * (a.H / (pack ? a.repeat : 1));
 }
 
-// Pieces of each tile's keys: where the tiles fill at most half of the CUs, as many as give each CU two
-// workgroups, of at least 256 keys.
+// Pieces of each tile's keys where the tiles fill at most half of the CUs: as many as give each CU a workgroup with
+// 256 keys (64 in float32, whose products take six times as long), or two with twice and four times that.  The
+// partials of every piece are written and read again, so more of them cost more than they give: B2 H32/8, 64 rows
+// over 4160 keys bf16 33 us with 8 pieces of 8 tiles, 37 with 16; B1 H32/8, 256 rows over 8192 keys 78 us with 4 and
+// 73 with 8; float32 B1 H8/2 E128, 20 rows over 500 keys 23 us with pieces of 64 keys, 53 with 256.
 int plan_splits(const WinArgs &a, bool bf16) {
     const int64_t blocks = blocks_of(a, packs(a)), cus = device_cus();
     if (blocks == 0 || cus <= 0 || 2 * blocks > cus) return 1;
-    const int BN = bf16 ? kKeys<__bf16> : kKeys<float>;
     const int64_t span = std::min<int64_t>(a.S, (int64_t)a.window + a.sinks + std::min(a.L, kM));
-    const int64_t most = std::max<int64_t>(1, span / std::max(256, BN));
-    return (int)std::min<int64_t>({most, 2 * cus / blocks, kMaxSplits});
+    const int64_t one = std::min<int64_t>(span / (bf16 ? 256 : 64), cus / blocks);
+    const int64_t two = std::min<int64_t>(span / (bf16 ? 512 : 256), 2 * cus / blocks);
+    return (int)std::min<int64_t>(std::max<int64_t>({one, two, 1}), kMaxSplits);
 }
 
 template <typename T, int D, bool VEC>
