@@ -316,7 +316,15 @@ def _dropout_apply(bits, x, scale):
 
 def _on(dev):
     """The launches of a call go to its tensors' device, whichever is current."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _like(t):
+    """A contiguous tensor like ``t``, not initialized (a third of the host time of ``torch.empty`` with a shape)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _unit_rows(t):
@@ -348,8 +356,8 @@ def _window_struct(*fields):
     return _lib.WindowDesc(*fields[:12], *(_strides(t) for t in fields[12:]))
 
 
-def _rotary_desc(q, k, inv_freq, positions, offset, interleaved, magnitude, eps, weights, grads=(None, None)):
-    """Checks the arguments of the rotation; returns its descriptor (``dc_rotary_desc``)."""
+def _rotary_fields(q, k, inv_freq, positions, offset, interleaved, magnitude, eps, weights, grads=(None, None)):
+    """Checks the arguments of the rotation; returns the fields of ``dc_rotary_desc`` but the strides."""
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("rotary takes (B, H, L, E) tensors")
     B, H, L, E = q.shape
@@ -387,43 +395,46 @@ def _rotary_desc(q, k, inv_freq, positions, offset, interleaved, magnitude, eps,
             raise ValueError("rotary takes positions or an offset, not both")
         pos_bytes = positions.element_size()
         ps = (positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0, positions.stride(-1))
-    return _rotary_struct(B, H, 0 if k is None else k.shape[1], L, E, 2 * inv_freq.shape[0], _DTYPES[q.dtype],
-                          _DTYPES[wdtype or q.dtype], interleaved, weights is not None, pos_bytes, 0,
-                          max(-2 ** 62, min(offset, 2 ** 62)), *ps,
-                          magnitude, eps, *(None if t is None else t.stride() for t in (q, k, *grads)))
+    return (B, H, 0 if k is None else k.shape[1], L, E, 2 * inv_freq.shape[0], _DTYPES[q.dtype],
+            _DTYPES[wdtype or q.dtype], interleaved, weights is not None, pos_bytes, 0,
+            max(-2 ** 62, min(offset, 2 ** 62)), *ps, magnitude, eps)
 
 
-def _rotary(q, k, inv_freq, positions=None, offset=0, interleaved=False, magnitude=1.0, weights=None, eps=0.0):
+def _rotary(q, k, inv_freq, positions=None, offset=0, interleaved=False, magnitude=1.0, weights=None, eps=0.0,
+            with_fields=False):
     """``dc_rotary_fwd``: (q, k) turned by their positions, contiguous; ``weights`` (a pair, either
-    None) asks for the norm of each head first.  ``k`` may be None."""
+    None) asks for the norm of each head first.  ``k`` may be None.  ``with_fields``: and what the backward
+    takes of the checks made here."""
     q, k = _unit_rows(q), None if k is None else _unit_rows(k)
     if weights is not None:
         weights = tuple(None if w is None else w.contiguous() for w in weights)
-    d = _rotary_desc(q, k, inv_freq, positions, offset, interleaved, magnitude, eps, weights)
+    fields = _rotary_fields(q, k, inv_freq, positions, offset, interleaved, magnitude, eps, weights)
+    d = _rotary_struct(*fields, q.stride(), None if k is None else k.stride(), None, None)
     inv_freq, dev = inv_freq.contiguous(), q.device
-    qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    ko = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+    qo, ko = _like(q), None if k is None else _like(k)
     wq, wk = weights or (None, None)
     with _on(dev):
         _lib.check(_lib.lib().dc_rotary_fwd(d, _ptr(q), _ptr(k), _ptr(wq), _ptr(wk), _ptr(inv_freq),
                                             _ptr(positions), _ptr(qo), _ptr(ko), _stream(dev)))
-    return qo, ko
+    return (qo, ko, fields) if with_fields else (qo, ko)
 
 
 def _rotary_backward(grad_q, grad_k, q, k, inv_freq, positions=None, offset=0, interleaved=False, magnitude=1.0,
-                     weights=None, eps=0.0, weight_grads=(False, False)):
+                     weights=None, eps=0.0, weight_grads=(False, False), fields=None):
     """``dc_rotary_bwd``: (dq, dk, dq_weight, dk_weight), None for what there is none of.  Without
-    ``weights`` q and k only give the shapes."""
+    ``weights`` q and k only give the shapes.  ``fields``: of the forward, whose arguments these are."""
     grad_q, grad_k = _unit_rows(grad_q), None if grad_k is None else _unit_rows(grad_k)
     if weights is not None:
         q, k = _unit_rows(q), None if k is None else _unit_rows(k)
         weights = tuple(None if w is None else w.contiguous() for w in weights)
-    d = _rotary_desc(q, k, inv_freq, positions, offset, interleaved, magnitude, eps, weights, (grad_q, grad_k))
+    if fields is None:
+        fields = _rotary_fields(q, k, inv_freq, positions, offset, interleaved, magnitude, eps, weights,
+                                (grad_q, grad_k))
     if grad_q.shape != q.shape or (k is not None and (grad_k is None or grad_k.shape != k.shape)):
         raise ValueError("rotary backward shapes do not match")
+    d = _rotary_struct(*fields, *(None if t is None else t.stride() for t in (q, k, grad_q, grad_k)))
     inv_freq, dev = inv_freq.contiguous(), q.device
-    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    dk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+    dq, dk = _like(q), None if k is None else _like(k)
     wq, wk = weights or (None, None)
     dwq, dwk = (torch.empty_like(w) if want and w is not None else None for w, want in zip((wq, wk), weight_grads))
     x = (q, k) if weights is not None else (None, None)
@@ -463,7 +474,7 @@ def _window_attention(q, k, v, window, sinks=0, offset=0, scale=None, with_rest=
     q, k, v = _unit_rows(q), _unit_rows(k), _unit_rows(v)
     d = _window_desc(q, k, v, window, sinks, offset, scale)
     dev, L_ = q.device, _lib.lib()
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out = _like(q)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
     rest = torch.empty_like(out) if with_rest and q.dtype == torch.bfloat16 else None
     with _on(dev):
@@ -485,7 +496,7 @@ def _window_attention_backward(grad_out, q, k, v, out, lse, rest, window, sinks=
     if rest is not None and (rest.shape != q.shape or rest.dtype != q.dtype or rest.device != dev):
         raise ValueError("window attention backward shapes do not match")
     out, lse, rest = out.contiguous(), lse.contiguous(), None if rest is None else rest.contiguous()
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v))
+    dq, dk, dv = _like(q), _like(k), _like(v)
     with _on(dev):
         ws = _scratch(L_.dc_window_bwd_workspace_size(d), dev)
         _lib.check(L_.dc_window_bwd(d, _ptr(grad_out), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(lse),
@@ -503,7 +514,7 @@ def _window_decode(q, k, v, window, sinks=0, lengths=None, scale=None):
                 or lengths.device != dev:
             raise ValueError("window decode lengths must be (B,) int32 or int64 on the tensors' device")
         lengths = lengths.contiguous()
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out = _like(q)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
     with _on(dev):
         ws = _scratch(L_.dc_window_decode_workspace_size(d), dev)

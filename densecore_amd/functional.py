@@ -340,8 +340,8 @@ def window_decode(query, key, value, window, sinks=0, lengths=None, scale=None):
     sequence b holds its first ``lengths[b]`` rows (int32 or int64 on the GPU; values are clamped to 0 .. S;
     None: all S), the query's own key the last of them.  Reads the visible rows alone; a sequence of
     length 0 gives 0.  Head dims up to 256, any strides; forward only."""
-    _check_tensors("attention", query=query, key=key, value=value,
-                   **({} if lengths is None else {"lengths": lengths}))
+    _check_tensors("attention", query=query, key=key, value=value)
+    _check_optional("attention", lengths=lengths)
     window, sinks, _, scale = _window_numbers(window, sinks, 0, scale)
     return _native._window_decode(query, key, value, window, sinks, lengths, scale)[0]
 
@@ -392,22 +392,23 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, wq, wk, norm, inv_freq, positions, args, eps):
-        weights = (wq, wk) if norm else None
+        qo, ko, fields = _native._rotary(q, k, inv_freq, positions, *args, (wq, wk) if norm else None, eps,
+                                         with_fields=True)
         ctx.save_for_backward(*(q, k, wq, wk) if norm else (None,) * 4, inv_freq, positions)
-        ctx.norm, ctx.args, ctx.eps, ctx.has_k = norm, args, eps, k is not None
-        ctx.like = [None if t is None else (t.shape, t.dtype, t.device) for t in (q, k)]
-        return _native._rotary(q, k, inv_freq, positions, *args, weights, eps)
+        ctx.norm, ctx.args, ctx.eps, ctx.fields, ctx.has_k = norm, args, eps, fields, k is not None
+        return qo, ko
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         q, k, wq, wk, inv_freq, positions = ctx.saved_tensors
+        gk = gk if ctx.has_k else None
         if not ctx.norm:
-            q, k = gq, gk if ctx.has_k else None
+            q, k = gq, gk
         need = ctx.needs_input_grad
         dq, dk, dwq, dwk = _native._rotary_backward(
-            gq, gk if ctx.has_k else None, q, k, inv_freq, positions, *ctx.args, (wq, wk) if ctx.norm else None,
-            ctx.eps, (need[2], need[3]))
+            gq, gk, q, k, inv_freq, positions, *ctx.args, (wq, wk) if ctx.norm else None, ctx.eps,
+            (need[2], need[3]), ctx.fields)
         return dq, dk, dwq, dwk, None, None, None, None, None
 
 
@@ -432,6 +433,10 @@ def _check_tensors(what, **tensors):
             raise TypeError(f"{what} {name} must be a Tensor")
 
 
+def _check_optional(what, **tensors):
+    _check_tensors(what, **{name: t for name, t in tensors.items() if t is not None})
+
+
 def rotary_embedding(query, key, inv_freq, positions=None, offset=0, interleaved=False, magnitude=1.0):
     """Queries (B, H, L, E) and keys (B, Hkv, L, E) turned by their positions: ``(query, key)``, contiguous.
 
@@ -441,8 +446,8 @@ def rotary_embedding(query, key, inv_freq, positions=None, offset=0, interleaved
     (2i, 2i + 1) when ``interleaved``; the dims behind them are passed on.  Float32 or bf16 in any strides
     (a projection's (B, L, H, E) is transposed on the way); angles are formed in float64.  ``key`` may be
     None: then the turned query alone is returned.  No counterpart in the reference."""
-    _check_tensors("rotary", query=query, inv_freq=inv_freq, **({} if key is None else {"key": key}),
-                   **({} if positions is None else {"positions": positions}))
+    _check_tensors("rotary", query=query, inv_freq=inv_freq)
+    _check_optional("rotary", key=key, positions=positions)
     args = _turn_args(offset, interleaved, magnitude)
     _refuse_frequency_gradient(inv_freq)
     if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
@@ -460,9 +465,8 @@ def qk_norm_rotary(query, key, query_weight, key_weight, inv_freq, positions=Non
     The weights are (E,) vectors, float32 or bf16, shared by the heads (None: no weight); with an empty
     ``inv_freq`` there is the norm alone.  Gradients: queries, keys and weights, the weights' summed in a
     fixed order.  No counterpart in the reference."""
-    _check_tensors("rotary", query=query, key=key, inv_freq=inv_freq,
-                   **({} if positions is None else {"positions": positions}),
-                   **{n: w for n, w in (("query_weight", query_weight), ("key_weight", key_weight)) if w is not None})
+    _check_tensors("rotary", query=query, key=key, inv_freq=inv_freq)
+    _check_optional("rotary", positions=positions, query_weight=query_weight, key_weight=key_weight)
     args = _turn_args(offset, interleaved, magnitude)
     _refuse_frequency_gradient(inv_freq)
     if isinstance(eps, bool) or not isinstance(eps, numbers.Real):
