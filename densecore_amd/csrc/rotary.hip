@@ -11,7 +11,9 @@
 // are wrong by 2^-4 at a position of 2^20).  Both are then Taylor sums in float32 (below).  A group keeps
 // its token's angles over `hb` heads, so they cost a tenth of the loads' time.
 //
-// Bound: HBM, each value in and out once.
+// Bound: HBM, each value in and out once (the norm's gradient reads x again).  B2 H32/8 L8192 E128 bf16: rotation
+// 66 us (335 MB, 5.1 TB/s; a copy of 2 GiB runs at 4.86), with norm 68, the norm's gradient 104 (503 MB, 4.8
+// TB/s).  One token: 4 us, a launch's latency.
 #include <algorithm>
 
 #include "common.hpp"

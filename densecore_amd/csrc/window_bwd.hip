@@ -3,8 +3,12 @@
 //     dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO,
 // dK and dV summed over the query heads that share a kv head.  Two kernels, no atomics:
 //   * window_dq_kernel (queries stay, the forward's structure) also forms dsum;
-//   * window_dkdv_kernel (keys stay): a workgroup of 4 waves owns 128 keys, 32 per wave with K and V in
-//     registers, and walks the queries that see one of them, head after head.
+//   * window_dkdv_kernel (keys stay): a workgroup owns 128 keys, 32 per wave, and walks the queries that see one
+//     of them, head after head; eight waves, where they fit, halve each step's queries and join at the end.
+// Bound: as the forward, a wave's own chain at two waves to a SIMD.  B2 H32/8 L8192 E128 W1024 with 4 sinks bf16:
+// dQ 599 us (650 TFLOP/s of the visible pairs' three products, 860 with dS's lo terms; MFMA busy 45%), dK and dV 1016 us
+// (510 of four products, 760 with lo terms; 38%), the sinks' pieces joined in 11.  Float32 B8 H12 L1024 E64 W256: 99,
+// 141 and 9 us.
 // Rows whose result is not finite are computed again in plain float32 over their visible pairs (as in
 // the forward, matrix products spread NaN and infinities to rows that do not see them).
 #include <algorithm>
@@ -489,7 +493,9 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, int rows) {
 
 // How the dK / dV grid is cut.  A tile of sinks has the queries of the whole sequence where the others have a
 // window's: pieces of about as many steps as those.  And where the blocks do not fill the CUs, pieces
-// of at least 4 steps that do.
+// of at least 4 steps that do.  bf16 E128: a step of B2 H32/8 L8192 W1024 with 4 sinks took 6.5 ms with a sink
+// tile's queries in one workgroup and 2.5 in pieces; the gradient of B1 H8/2 L1024 W256 90 us without pieces or with
+// pieces of 16 steps, 56 with those of 4.
 void plan_pieces(WinArgs &a, bool bf16) {
     const int QM = 32 * (bf16 || a.E <= 64 ? 2 : 1), nkt = (a.S + kM - 1) / kM;
     a.sink_tiles = (int)std::min<int64_t>(nkt, ((int64_t)a.sinks + kM - 1) / kM);

@@ -1,5 +1,6 @@
 // One query per sequence over a KV cache with a window and sinks (dc_window_decode): bound by reading the
-// visible rows of K and V once.
+// visible rows of K and V once.  Float32 B8 H32/8 E128, 4096 keys: 51 us, 5.2 TB/s; bf16 B16: 57 us for a call, its two
+// kernels 45 + 5 (269 MB, 6.0 TB/s in the first).
 //
 // A cache row belongs to LPR lanes, each with one 16-byte piece; a wave reads 64 / LPR rows at a time, U
 // times over, K and V together.  The REP query heads of a workgroup share those registers.  A group of
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(kThreads) void window_decode_kernel(WinDecodeArgs a
 // bf16 (16-byte pieces, head dims up to 128): the same, with the products on the matrix cores, so that the heads
 // sharing a row (up to 16) cost next to nothing: 8 heads to a kv head are 150 VALU instructions for each 16 bytes
 // of K and V in the kernel above, which is then bound by them (B8 H64/8 E128, 8192 keys: 148 us, here 51;
-// B16 H32/8 over the last 4096 keys 67 and 53, 5.0 TB/s).
+// B16 H32/8 over the last 4096 keys 67 and 53).
 //
 // A wave takes 32 keys at a time on its own, no barrier: K and V rows come by global_load_lds into its two
 // buffers, whole rows by neighbouring lanes, their 16-byte chunks xored with the row so that neither the reads of
