@@ -25,9 +25,14 @@ constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // dQ: keys per tile
 // Two waves per SIMD or more, but for float32 at D = 128 (three parts of two operands and the sums take 350 registers).
 template <typename T, int D>
 constexpr int kWavesPerSimd = sizeof(T) == 2 || D <= 64 ? 2 : 1;
-// dK / dV: waves w and w + 4 own the same 32 keys and halve each step's queries (one wave per SIMD: no halves).
+// dK / dV: with two halves, waves w and w + 4 own the same 32 keys and halve each step's queries, one workgroup to a
+// CU (its tiles fill the LDS); with one, several workgroups share a CU and a wave has twice the products between two
+// barriers: B4 H32 L4096 W1024 bf16 E64 backward 884 us with halves, 765 without, E32 565 and 444 (three waves per SIMD);
+// float32 E32 433 and 390, while at E64 keeping V in registers for it spills (239 and 256).
 template <typename T, int D>
-constexpr int kHalves = kWavesPerSimd<T, D>;
+constexpr int kHalves = D == 32 || (sizeof(T) == 2 && D == 64) ? 1 : kWavesPerSimd<T, D>;
+template <typename T, int D>
+constexpr int kQueries = sizeof(T) == 2 || D <= 64 ? 64 : 32;  // per step
 // dK / dV: K's, V's operands in LDS and not in registers, where these would spill (at D = 128 the sums alone
 // take half of bf16's, and float32's take 350 with one wave per SIMD).
 template <typename T, int D>
@@ -226,7 +231,7 @@ template <typename T, int D, bool VEC>
 __global__ __launch_bounds__((kThreads * kHalves<T, D>))
 __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dkdv_kernel(WinArgs a) {
     typedef Ops<T> O;
-    constexpr int HALVES = kHalves<T, D>, QM = 32 * HALVES, THREADS = kThreads * HALVES, KSTEP = D / 16, NDT = D / 32;
+    constexpr int HALVES = kHalves<T, D>, QM = kQueries<T, D>, THREADS = kThreads * HALVES, KSTEP = D / 16, NDT = D / 32;
     constexpr bool KLDS = kKLds<T, D>, VLDS = kVLds<T, D>;
     typedef Stage<T, QM, D, THREADS, VEC> St;
     typedef Stage<T, VLDS ? kM : 32, D, THREADS, VEC> StV;
@@ -237,7 +242,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dkdv_kerne
     };
     union Smem {
         Main m;
-        float red[HALVES - 1][kWaves][NDT][16][64];  // the second half's sums on their way to the first
+        float red[HALVES > 1][kWaves][NDT][16][64];  // the second half's sums on their way to the first
     };
     __shared__ Smem sm;
 
@@ -317,8 +322,8 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dkdv_kerne
     const uint32_t rowb = row_lanebase<QM, D>(lane), trb = tr_lanebase<QM, D>(lane);
     const uint32_t rowk = row_lanebase<VLDS ? kM : 32, D>(lane);
 
-    auto step = [&](int i, At x) {
-        const int buf = i & 1, mq = x.m + 32 * half, r0 = 32 * half;
+    auto step = [&](int i, At x, int part) {
+        const int buf = i & 1, mq = x.m + 32 * part, r0 = 32 * part;
         const int q0 = a.offset + mq, q1 = a.offset + min(mq + 31, a.L - 1);
         if (mq >= a.L || kw0 >= a.S || kw0 > q1 || (q0 - (kw0 + 31) >= a.window && kw0 >= a.sinks)) return;
         const bool all = kw0 + 31 < a.S && kw0 + 31 <= q0 && (q1 - kw0 < a.window || kw0 + 31 < a.sinks);
@@ -382,7 +387,12 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dkdv_kerne
         __syncthreads();
         const At then = next(now);
         if (i + 1 < i1) start(i + 1, then);
-        step(i, now);
+        if constexpr (32 * HALVES == QM) {
+            step(i, now, half);
+        } else {
+#pragma unroll 1
+            for (int part = 0; part < QM / 32; ++part) step(i, now, part);
+        }
         if (i + 1 < i1) finish(i + 1, then);
         now = then;
     }
@@ -497,7 +507,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, int rows) {
 // tile's queries in one workgroup and 2.5 in pieces; the gradient of B1 H8/2 L1024 W256 90 us without pieces or with
 // pieces of 16 steps, 56 with those of 4.
 void plan_pieces(WinArgs &a, bool bf16) {
-    const int QM = 32 * (bf16 || a.E <= 64 ? 2 : 1), nkt = (a.S + kM - 1) / kM;
+    const int QM = bf16 || a.E <= 64 ? 64 : 32, nkt = (a.S + kM - 1) / kM;
     a.sink_tiles = (int)std::min<int64_t>(nkt, ((int64_t)a.sinks + kM - 1) / kM);
     a.sink_pieces = a.tile_pieces = 1;
     if (nkt == 0 || a.L == 0 || a.B * a.Hkv == 0) return;
