@@ -4,7 +4,7 @@
 // dK and dV summed over the query heads that share a kv head.  Two kernels, no atomics:
 //   * window_dq_kernel (queries stay, the forward's structure) also forms dsum;
 //   * window_dkdv_kernel (keys stay): a workgroup owns 128 keys, 32 per wave, and walks the queries that see one
-//     of them, head after head; eight waves, where they fit, halve each step's queries and join at the end.
+//     of them, head after head; where its tiles fill the LDS, eight waves halve each step's queries and join at the end.
 // Bound: as the forward, a wave's own chain at two waves to a SIMD.  B2 H32/8 L8192 E128 W1024 with 4 sinks bf16:
 // dQ 599 us (650 TFLOP/s of the visible pairs' three products, 860 with dS's lo terms; MFMA busy 45%), dK and dV 1016 us
 // (510 of four products, 760 with lo terms; 38%), the sinks' pieces joined in 11.  Float32 B8 H12 L1024 E64 W256: 99,

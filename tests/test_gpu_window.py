@@ -672,3 +672,31 @@ def test_gradient_pieces(sizes):
     ref = formulas(q, k, v, open_, 32 ** -0.5, torch.float32, g)
     for name, x in (("out", y), ("dq", dq), ("dk", dk), ("dv", dv)):
         close(x, *ref[name], torch.float32, name)
+
+
+def _random_case(seed):
+    import random
+    r = random.Random(seed)
+    Hkv, rep = r.choice([1, 2, 3, 5]), r.choice([1, 1, 2, 3, 4, 8])
+    E = r.choice([8, 16, 24, 32, 40, 48, 64, 64, 72, 96, 128, 128, r.randint(1, 128)])
+    S = r.choice([r.randint(1, 70), r.randint(60, 400), r.randint(400, 1500)])
+    L = r.choice([1, 2, r.randint(1, 70), min(S, 300), r.randint(60, 300)])
+    offset = r.choice([0, max(S - L, 0), max(S - L, 0), r.randint(0, 2 * S)])
+    window = r.choice([1, r.randint(1, 40), r.randint(30, 300), S, 5 * S])
+    sinks = r.choice([0, 0, 1, 4, r.randint(0, 200)])
+    return r.randint(1, 3), Hkv * rep, Hkv, L, S, E, window, sinks, offset
+
+
+@TYPES
+@pytest.mark.parametrize("seed", range(40))
+def test_random_sizes(seed, dtype):
+    test_forward_and_gradients(_random_case(seed), dtype)
+
+
+@TYPES
+@pytest.mark.parametrize("seed", range(30))
+def test_decode_of_random_sizes(seed, dtype):
+    import random
+    r = random.Random(seed)
+    B, H, Hkv, _, S, E, window, sinks, _ = _random_case(1000 + seed)
+    test_decode((B, H, Hkv, S, r.choice([E, 2 * E]), window, sinks, r.choice([None, [r.randint(0, S) for _ in range(B)]])), dtype)
