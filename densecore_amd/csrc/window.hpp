@@ -68,6 +68,9 @@ namespace {
 // Whether the query at position p sees key s (s < S is the caller's).
 DEVI bool sees(int p, int s, int window, int sinks) { return s <= p && (p - s < window || s < sinks); }
 
+// Whether it sees any key at all.
+DEVI bool sees_any(const WinArgs &a, int p) { return a.S > 0 && (a.sinks > 0 || p - a.window < a.S - 1); }
+
 // Which of the keys base + c a query at p sees (c a constant): three compares, no branch.
 struct SeenKeys {
     int hi, lo, sink;

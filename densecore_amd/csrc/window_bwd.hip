@@ -179,7 +179,10 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dq_kernel(
         const float rlse = a.lse_in[rr];
         if (lane == 0) a.dsum[rr] = rs;
         float o[2] = {0.f, 0.f};
-        for (int i = 0; i < band.n; ++i) {
+        // (The same in all lanes.)  A NaN lse or dsum is in every dS of the row.
+        const bool lost = (rlse != rlse || rs != rs) && sees_any(a, rp);
+        if (lost) o[0] = o[1] = NAN;
+        for (int i = 0; i < band.n && !lost; ++i) {
             const int n0 = band.tile(i) * BN, key = n0 + lane;
             const bool ok = lane < BN && key < a.S && sees(rp, key, a.window, a.sinks);
             float ds = 0.f;
@@ -449,7 +452,15 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dkdv_kerne
         const int ra = 32 * kw + __builtin_ctz(again), rk = n0 + ra;
         const T *k1 = kb + rk * a.ks[2], *v1 = vb + rk * a.vs[2];
         float xk[2] = {0.f, 0.f}, xv[2] = {0.f, 0.f};
-        for (int i = i0; i < i1; ++i) {
+        bool lost = false;  // a query that sees the key has a NaN lse: so are its P and this key's sums
+        for (int i = i0; i < i1 && !lost; ++i) {
+            const int h = hk * a.repeat + i / per_head, l = l0 + i % per_head * QM + lane;
+            const bool ok = lane < QM && l < a.L && sees(a.offset + l, rk, a.window, a.sinks);
+            const float lse = ok ? a.lse_in[((int64_t)b * a.H + h) * a.L + l] : 0.f;
+            lost = __any(lse != lse);
+        }
+        if (lost) xk[0] = xk[1] = xv[0] = xv[1] = NAN;
+        for (int i = i0; i < i1 && !lost; ++i) {
             const int h = hk * a.repeat + i / per_head, m = l0 + i % per_head * QM, l = m + lane;
             const bool ok = lane < QM && l < a.L && sees(a.offset + l, rk, a.window, a.sinks);
             float pr = 0.f, ds = 0.f;

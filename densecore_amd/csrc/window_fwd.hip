@@ -71,6 +71,10 @@ DEVI void plain_row(const WinArgs &a, const T *q, const T *kb, const T *vb, int 
         const float top = fmaxf(m, wave_max(s)), base = top == -INFINITY ? 0.f : top;
         sum = sum * exp2_fast(m - base) + wave_sum(ok ? exp2_fast(s - base) : 0.f);
         m = top;
+        if (sum != sum) {  // a score that is seen is NaN: so is the row, whatever follows
+            o[0] = o[1] = sum;
+            return;
+        }
     }
     const float base = m == -INFINITY ? 0.f : m, inv = sum == 0.f ? 0.f : 1.f / sum;
     for (int i = i0; i < i1; ++i) {

@@ -700,3 +700,47 @@ def test_decode_of_random_sizes(seed, dtype):
     r = random.Random(seed)
     B, H, Hkv, _, S, E, window, sinks, _ = _random_case(1000 + seed)
     test_decode((B, H, Hkv, S, r.choice([E, 2 * E]), window, sinks, r.choice([None, [r.randint(0, S) for _ in range(B)]])), dtype)
+
+
+@TYPES
+@pytest.mark.parametrize("what", ["all", "queries", "keys", "values", "gradients", "some"])
+def test_results_that_are_not_finite(what, dtype):
+    """NaN where the formulas have it and nowhere else: rows that see no key stay 0, the others' hidden
+    neighbours finite; sinks, pieces of keys and a few rows over many keys among them."""
+    from densecore_amd import functional as F
+    gen = torch.Generator().manual_seed(41)
+    for B, H, Hkv, L, S, E, window, sinks, offset in ((1, 4, 2, 400, 400, 64, 70, 4, 0), (2, 2, 1, 260, 200, 40, 30, 0, 0),
+                                                      (1, 4, 1, 9, 1500, 128, 900, 3, 1491)):
+        q, k, v, g = (torch.randn(B, h, n, E, generator=gen).to(dtype).to(DEV) for h, n in ((H, L), (Hkv, S), (Hkv, S), (H, L)))
+        for name, t in (("queries", q), ("keys", k), ("values", v), ("gradients", g)):
+            if what in ("all", name):
+                t.fill_(math.nan)
+            elif what == "some":
+                t[:, :, t.shape[2] // 2] = math.nan
+        open_ = visible(offset + torch.arange(L, device=DEV), S, window, sinks)
+        leaves = [t.requires_grad_(True) for t in (q, k, v)]
+        y = F.window_attention(*leaves, window, sinks, offset)
+        dq, dk, dv = torch.autograd.grad(y, leaves, g)
+
+        def dirty(t):  # rows, (B, H, rows)
+            return torch.isnan(t.detach().float()).any(-1)
+
+        def shared(t):
+            return t.repeat_interleave(H // Hkv, 1)
+        pair = open_[None, None]
+        q_, k_, v_, g_ = dirty(q), shared(dirty(k)), shared(dirty(v)), dirty(g)
+        score = pair & (q_[..., None] | k_[:, :, None])          # pairs whose score is NaN
+        row = score.any(-1)                                      # rows whose P is NaN
+        out = row | (pair & v_[:, :, None]).any(-1)
+        sees = open_.any(-1)[None, None].expand(B, H, L)
+        ds = sees & (out | g_)                                   # dsum takes both
+        p_pair, ds_pair = pair & row[..., None], pair & (ds[..., None] | v_[:, :, None])
+
+        def group(t):
+            return t.reshape(B, Hkv, H // Hkv, S).any(2)
+        want = {"out": out, "dq": (ds_pair | (pair & k_[:, :, None])).any(-1),
+                "dk": group((ds_pair | (pair & q_[..., None])).any(2)), "dv": group((p_pair | (pair & g_[..., None])).any(2))}
+        for name, t in (("out", y), ("dq", dq), ("dk", dk), ("dv", dv)):
+            assert torch.equal(torch.isnan(t).all(-1), want[name]), (name, L)
+            assert torch.equal(torch.isnan(t).any(-1), want[name]), (name, L)
+        assert not y[~sees].any() and not dq[~sees].any()
