@@ -332,6 +332,11 @@ DEVI float plain_dot(const T *a, const T *b, int E) {
     return s;
 }
 
+// Whether a row's E dims, in lanes' x0 and x1 (dims lane and lane + 64), are all NaN: nothing added changes them.
+DEVI bool all_nan(int lane, int E, float x0, float x1) {
+    return __all((lane >= E || x0 != x0) && (lane + 64 >= E || x1 != x1));
+}
+
 DEVI float wave_max(float x) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o, 64));

@@ -197,6 +197,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dq_kernel(
                 if (lane < a.E) o[0] = fmaf(dj, to_f32<T>(k1[lane]), o[0]);
                 if (lane + 64 < a.E) o[1] = fmaf(dj, to_f32<T>(k1[lane + 64]), o[1]);
             }
+            if (all_nan(lane, a.E, o[0], o[1])) break;
         }
         if (lane < a.E) dq[rr * a.E + lane] = from_f32<T>(o[0] * a.scale);
         if (lane + 64 < a.E) dq[rr * a.E + lane + 64] = from_f32<T>(o[1] * a.scale);
@@ -477,6 +478,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dkdv_kerne
                 for (int d = lane, n = 0; n < 2; ++n, d += 64)
                     if (d < a.E) xk[n] = fmaf(dj, to_f32<T>(q1[d]), xk[n]), xv[n] = fmaf(pj, to_f32<T>(g1[d]), xv[n]);
             }
+            if (all_nan(lane, a.E, xk[0], xk[1]) && all_nan(lane, a.E, xv[0], xv[1])) break;
         }
 #pragma unroll
         for (int d = lane, n = 0; n < 2; ++n, d += 64)

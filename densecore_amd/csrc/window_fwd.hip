@@ -87,6 +87,7 @@ DEVI void plain_row(const WinArgs &a, const T *q, const T *kb, const T *vb, int 
             if (lane < a.E) o[0] = fmaf(pj, to_f32<T>(v[lane]), o[0]);
             if (lane + 64 < a.E) o[1] = fmaf(pj, to_f32<T>(v[lane + 64]), o[1]);
         }
+        if (all_nan(lane, a.E, o[0], o[1])) return;
     }
 }
 
