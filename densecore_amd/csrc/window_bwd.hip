@@ -421,47 +421,45 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dkdv_kerne
         join(dk), join(dv);
         if (half == 1) return;
     }
-    float test = 0.f;
+    float testk = 0.f, testv = 0.f;
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) test += not_finite(dk[dt]) + not_finite(dv[dt]);
-    const uint64_t wrong = __ballot(key < a.S && test != 0.f);
-    uint32_t again = (uint32_t)wrong | (uint32_t)(wrong >> 32);
+    for (int dt = 0; dt < NDT; ++dt) testk += not_finite(dk[dt]), testv += not_finite(dv[dt]);
+    const uint64_t wrongk = __ballot(key < a.S && testk != 0.f), wrongv = __ballot(key < a.S && testv != 0.f);
+    const uint32_t againk = (uint32_t)wrongk | (uint32_t)(wrongk >> 32), againv = (uint32_t)wrongv | (uint32_t)(wrongv >> 32);
     // Rows of this block: results, or its piece's float32 slot.
     T *dko = static_cast<T *>(a.dk) + ((int64_t)bhk * a.S + n0) * a.E, *dvo = static_cast<T *>(a.dv) + ((int64_t)bhk * a.S + n0) * a.E;
     float *pk = a.kv_part + (pcs.slot + piece) * 2 * kM * a.E, *pv = pk + (int64_t)kM * a.E;
     const int at = 32 * kw + lr;
-    if (key < a.S && !((again >> lr) & 1)) {
+    auto put = [&](const f32x16 (&x)[NDT], float scale, T *out, float *part) {
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const int d = dt * 32 + acc_row(e, g);
-                float x[4], y[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = dk[dt][e + j] * a.scale, y[j] = dv[dt][e + j];
-                if (pcs.n > 1) {
-                    store4<float, VEC>(pk + at * a.E, d, a.E, x[0], x[1], x[2], x[3]);
-                    store4<float, VEC>(pv + at * a.E, d, a.E, y[0], y[1], y[2], y[3]);
-                } else {
-                    store4<T, VEC>(dko + (int64_t)at * a.E, d, a.E, x[0], x[1], x[2], x[3]);
-                    store4<T, VEC>(dvo + (int64_t)at * a.E, d, a.E, y[0], y[1], y[2], y[3]);
-                }
+                const float x0 = x[dt][e] * scale, x1 = x[dt][e + 1] * scale, x2 = x[dt][e + 2] * scale, x3 = x[dt][e + 3] * scale;
+                if (pcs.n > 1) store4<float, VEC>(part + at * a.E, d, a.E, x0, x1, x2, x3);
+                else store4<T, VEC>(out + (int64_t)at * a.E, d, a.E, x0, x1, x2, x3);
             }
-    }
+    };
+    if (key < a.S && !((againk >> lr) & 1)) put(dk, a.scale, dko, pk);
+    if (key < a.S && !((againv >> lr) & 1)) put(dv, 1.f, dvo, pv);
     // Keys again, over this block's steps: lanes are queries for P and dS and dims for the sums.
-    for (; again; again &= again - 1) {
-        const int ra = 32 * kw + __builtin_ctz(again), rk = n0 + ra;
+    for (uint32_t again = againk | againv; again; again &= again - 1) {
+        const int bit = __builtin_ctz(again), ra = 32 * kw + bit, rk = n0 + ra;
+        const bool wantk = (againk >> bit) & 1, wantv = (againv >> bit) & 1;
         const T *k1 = kb + rk * a.ks[2], *v1 = vb + rk * a.vs[2];
-        float xk[2] = {0.f, 0.f}, xv[2] = {0.f, 0.f};
-        bool lost = false;  // a query that sees the key has a NaN lse: so are its P and this key's sums
-        for (int i = i0; i < i1 && !lost; ++i) {
+        // A NaN lse of a query that sees the key is in P, it and a NaN dsum in dS: the key's sums are NaN.
+        bool lostk = !wantk, lostv = !wantv;
+        for (int i = i0; i < i1 && !(lostk && lostv); ++i) {
             const int h = hk * a.repeat + i / per_head, l = l0 + i % per_head * QM + lane;
             const bool ok = lane < QM && l < a.L && sees(a.offset + l, rk, a.window, a.sinks);
-            const float lse = ok ? a.lse_in[((int64_t)b * a.H + h) * a.L + l] : 0.f;
-            lost = __any(lse != lse);
+            const int64_t row = ((int64_t)b * a.H + h) * a.L + l;
+            const float lse = ok ? a.lse_in[row] : 0.f, rs = ok ? a.dsum[row] : 0.f;
+            lostv |= (bool)__any(lse != lse), lostk |= (bool)__any(lse != lse || rs != rs);
         }
-        if (lost) xk[0] = xk[1] = xv[0] = xv[1] = NAN;
-        for (int i = i0; i < i1 && !lost; ++i) {
+        float xk[2], xv[2];
+        xk[0] = xk[1] = lostk ? NAN : 0.f, xv[0] = xv[1] = lostv ? NAN : 0.f;
+        for (int i = i0; i < i1 && !(all_nan(lane, a.E, xk[0], xk[1]) && all_nan(lane, a.E, xv[0], xv[1])); ++i) {
             const int h = hk * a.repeat + i / per_head, m = l0 + i % per_head * QM, l = m + lane;
             const bool ok = lane < QM && l < a.L && sees(a.offset + l, rk, a.window, a.sinks);
             float pr = 0.f, ds = 0.f;
@@ -478,18 +476,19 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dkdv_kerne
                 for (int d = lane, n = 0; n < 2; ++n, d += 64)
                     if (d < a.E) xk[n] = fmaf(dj, to_f32<T>(q1[d]), xk[n]), xv[n] = fmaf(pj, to_f32<T>(g1[d]), xv[n]);
             }
-            if (all_nan(lane, a.E, xk[0], xk[1]) && all_nan(lane, a.E, xv[0], xv[1])) break;
         }
 #pragma unroll
-        for (int d = lane, n = 0; n < 2; ++n, d += 64)
-            if (d < a.E) {
-                if (pcs.n > 1) {
-                    pk[ra * a.E + d] = xk[n] * a.scale, pv[ra * a.E + d] = xv[n];
-                } else {
-                    dko[(int64_t)ra * a.E + d] = from_f32<T>(xk[n] * a.scale);
-                    dvo[(int64_t)ra * a.E + d] = from_f32<T>(xv[n]);
-                }
+        for (int d = lane, n = 0; n < 2; ++n, d += 64) {
+            if (d >= a.E) continue;
+            if (wantk) {
+                if (pcs.n > 1) pk[ra * a.E + d] = xk[n] * a.scale;
+                else dko[(int64_t)ra * a.E + d] = from_f32<T>(xk[n] * a.scale);
             }
+            if (wantv) {
+                if (pcs.n > 1) pv[ra * a.E + d] = xv[n];
+                else dvo[(int64_t)ra * a.E + d] = from_f32<T>(xv[n]);
+            }
+        }
     }
 }
 
