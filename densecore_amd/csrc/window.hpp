@@ -321,6 +321,34 @@ DEVI void store4(T *row, int d, int E, float x0, float x1, float x2, float x3) {
     }
 }
 
+// A wave's 32 rows of results, value(dt, e) of its lanes' accumulators (rows on lanes), to the rows that row(r) gives (null:
+// none), turned in LDS so that neighbouring lanes write neighbouring 16-byte pieces.  `room`: kRoom<D> pieces, the wave's own.
+// A lane's own 8 bytes of each row otherwise: B2 H32/8 L8192 E128 W1024 forward with the rest 532 us, turned 515; W128 229 and
+// 207, dQ 313 and 302; at E64 and below it takes as long or longer, and in dK / dV the registers (1023 and 1151).
+template <typename T, int D, bool VEC>
+constexpr bool kTurned = sizeof(T) == 2 && D == 128 && VEC;
+template <int D>
+constexpr int kRoom = 32 * (D / 8 + 1);
+template <int D, typename Value, typename Row>
+DEVI void store_turned(u32x4 *room, int lane, int E, Value value, Row row) {
+    constexpr int C = D / 8, P = C + 1;
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+            reinterpret_cast<u32x2 *>(room + (lane & 31) * P + 4 * dt + e / 4)[lane >> 5] =
+                u32x2{cvt_pk_bf16(value(dt, e), value(dt, e + 1)), cvt_pk_bf16(value(dt, e + 2), value(dt, e + 3))};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < C / 2; ++i) {
+        const int r = (64 * i + lane) / C, c = (64 * i + lane) % C;
+        __bf16 *to = row(r);
+        if (to && 8 * c < E) *reinterpret_cast<u32x4 *>(to + 8 * c) = room[r * P + c];
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // before the room is written again
+}
+
 // What rounding x to bf16 leaves.
 DEVI float rest_of(float x) { return x - bf16_to_f32(f32_to_bf16(x)); }
 

@@ -47,6 +47,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dq_kernel(
     constexpr int BN = kKeys<T>, NT = BN / 32, KSTEP = D / 16, NDT = D / 32;
     typedef Stage<T, BN, D, kThreads, VEC> St;
     __shared__ typename St::Tile sk[2], sv[2];
+    static_assert(!kTurned<T, D, VEC> || sizeof(sk) >= kWaves * kRoom<D> * sizeof(u32x4), "the results' turn");
 
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -161,7 +162,13 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_dq_kernel(
     const uint64_t wrong = __ballot(in && test != 0.f);
     uint32_t again = (uint32_t)wrong | (uint32_t)(wrong >> 32);
     T *dq = static_cast<T *>(a.dq);
-    if (in && !((again >> lr) & 1)) {
+    if constexpr (kTurned<T, D, VEC>) {
+        __syncthreads();  // everyone is done with the tiles, which the results now pass through
+        store_turned<D>(reinterpret_cast<u32x4 *>(sk) + wave * kRoom<D>, lane, a.E,
+                        [&](int dt, int e) { return acc[dt][e] * a.scale; }, [&](int r1) -> __bf16 * {
+                            return wr0 + r1 < a.L && !((again >> r1) & 1) ? dq + ((int64_t)bh * a.L + wr0 + r1) * a.E : nullptr;
+                        });
+    } else if (in && !((again >> lr) & 1)) {
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll

@@ -8,7 +8,7 @@
 // each head that shares a kv head) are packed into one tile.
 //
 // Bound: a wave's own chain of transfers, products and softmax, two waves to a SIMD.  B2 H32/8 L8192 E128 W1024 bf16:
-// 448 us, and 521 with the rest written, 500 TFLOP/s of the visible pairs' 4 E and 750 with P's lo terms (a library
+// 440 us, and 515 with the rest written, 500 TFLOP/s of the visible pairs' 4 E and 750 with P's lo terms (a library
 // product of 8192^3 reaches 1139); MFMA busy 38%.  At a step that took 488 us, leaving out the maximum gave 474,
 // the exponentials 425, P V 357, the transfers 385: no single one of them is what a wave waits for.  Float32 (six bf16
 // products each) B8 H12 L1024 E64 W256: 76 us.
@@ -95,7 +95,7 @@ DEVI void plain_row(const WinArgs &a, const T *q, const T *kb, const T *vb, int 
 // or the piece's share of them; rows that are not finite again.
 template <typename T, int D, bool VEC>
 DEVI void write_rows(const WinArgs &a, const f32x16 (&acc)[D / 32], float m_run, float l_part, int lane, int wr0, bool in,
-                     int64_t row, int b, int h0, const T *kb, const T *vb, Band band, int i0, int i1, int piece) {
+                     int64_t row, int b, int h0, const T *kb, const T *vb, Band band, int i0, int i1, int piece, void *room) {
     constexpr int NDT = D / 32;
     const int lr = lane & 31, g = lane >> 5;
     const float l_run = xor32_add(l_part);
@@ -107,6 +107,21 @@ DEVI void write_rows(const WinArgs &a, const f32x16 (&acc)[D / 32], float m_run,
     const uint64_t wrong = __ballot(in && test != 0.f);
     uint32_t again = (uint32_t)wrong | (uint32_t)(wrong >> 32);
     const int64_t nrows = (int64_t)a.B * a.H * a.L;
+    if constexpr (kTurned<T, D, VEC>) {
+        if (a.splits == 1) {
+            const int rows = (a.pack ? a.repeat : 1) * a.L;
+            auto to = [&](void *base) {
+                return [&, base](int r) -> __bf16 * {
+                    if (wr0 + r >= rows || ((again >> r) & 1)) return nullptr;
+                    const RowAt ra = row_at(a, wr0 + r);
+                    return static_cast<__bf16 *>(base) + (((int64_t)b * a.H + h0 + ra.h) * a.L + ra.l) * a.E;
+                };
+            };
+            u32x4 *const turn = static_cast<u32x4 *>(room);
+            store_turned<D>(turn, lane, a.E, [&](int dt, int e) { return acc[dt][e] * inv; }, to(a.out));
+            if (a.rest) store_turned<D>(turn, lane, a.E, [&](int dt, int e) { return rest_of(acc[dt][e] * inv); }, to(a.rest));
+        }
+    }
     if (in && !((again >> lr) & 1)) {
         const float lse = (m_run + log2_fast(l_run)) * kLn2;
         if (a.splits > 1) {
@@ -119,6 +134,7 @@ DEVI void write_rows(const WinArgs &a, const f32x16 (&acc)[D / 32], float m_run,
                                        acc[dt][e + 2] * inv, acc[dt][e + 3] * inv);
             if (g == 0) a.part_lse[slot] = empty ? -INFINITY : lse;
         } else {
+            if constexpr (!kTurned<T, D, VEC>) {
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -131,6 +147,7 @@ DEVI void write_rows(const WinArgs &a, const f32x16 (&acc)[D / 32], float m_run,
                         store4<T, VEC>(static_cast<T *>(a.rest) + row * a.E, d, a.E, rest_of(x0), rest_of(x1), rest_of(x2),
                                        rest_of(x3));
                 }
+            }
             if (g == 0) a.lse[row] = empty ? 0.f : lse;
         }
     }
@@ -164,6 +181,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_fwd_kernel
     constexpr int BN = kKeys<T>, NT = BN / 32, KSTEP = D / 16, NDT = D / 32;
     typedef Stage<T, BN, D, kThreads, VEC> St;
     __shared__ typename St::Tile sk[2], sv[2];
+    static_assert(!kTurned<T, D, VEC> || sizeof(sk) >= kWaves * kRoom<D> * sizeof(u32x4), "the results' turn");
 
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -313,7 +331,9 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D>))) void window_fwd_kernel
         if (i + 1 < i1) finish(i + 1);
     }
 
-    write_rows<T, D, VEC>(a, acc, m_run, l_part, lane, wr0, in, row, b, h0, kb, vb, band, i0, i1, piece);
+    if (kTurned<T, D, VEC>) __syncthreads();  // everyone is done with the tiles, which the results now pass through
+    write_rows<T, D, VEC>(a, acc, m_run, l_part, lane, wr0, in, row, b, h0, kb, vb, band, i0, i1, piece,
+                          reinterpret_cast<u32x4 *>(sk) + wave * kRoom<D>);
 }
 
 // Joins the pieces of each row, 16 lanes per row: lse = log sum exp(lse_i), out = sum exp(lse_i - lse) o_i.
